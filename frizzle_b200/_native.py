@@ -62,6 +62,27 @@ class CaptureSlots(C.Structure):
                [(n, C.c_uint32) for n in ("keys", "query_heads", "window", "full_attention")]
 
 
+class PagedKv(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("keys", "values", "page_table", "lengths", "weights", "bounds", "error")] + \
+               [(n, C.c_uint64) for n in ("page_stride", "slot_stride", "head_stride")] + \
+               [(n, C.c_uint32) for n in ("sequences", "table_stride", "pages", "page_slots", "kv_heads", "head_dim",
+                                           "type", "padding")]
+
+
+class PagedRows(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out")] + \
+               [(n, C.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + \
+               [(n, C.c_void_p) for n in ("q_gain", "k_gain", "turns", "sequence", "index", "position")] + \
+               [("rows", C.c_uint32), ("heads", C.c_uint32), ("eps", C.c_float), ("padding", C.c_uint32)]
+
+
+class PagedQuery(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_uint64), ("out_stride", C.c_uint64),
+                ("blocks", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)] + \
+               [(n, C.c_uint32) for n in ("heads", "top", "window")] + \
+               [("scale", C.c_float), ("decay", C.c_float), ("padding", C.c_uint32)]
+
+
 # Every symbol the header declares, with its signature.
 VP = C.c_void_p
 U32 = C.c_uint32
@@ -127,6 +148,12 @@ SIGNATURES = {
     "fz_attention_splits": (U32, [U32, U32, U32]),
     "fz_attention_wide": (C.c_int, [VP, VP, VP, U32, U32, U32, U32, U32, U32, U32, VP, VP, VP, VP, VP, VP]),
     "fz_attention_static": (C.c_int, [VP, VP, VP, U32, U32, U32, U32, U32, U32, U32, VP, VP]),
+    "fz_paged_append": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedRows), VP]),
+    "fz_paged_bounds": (C.c_int, [C.POINTER(PagedKv), VP, VP]),
+    "fz_paged_select": (C.c_int, [C.POINTER(PagedKv), VP, C.c_uint64, U32, U32, U32, U32, VP, VP, VP]),
+    "fz_paged_attention": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedQuery), VP]),
+    "fz_paged_attention_workspace": (C.c_size_t, [C.POINTER(PagedKv), U32]),
+    "fz_paged_evict": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedKv), U32, U32, U32, VP, VP]),
 }
 
 

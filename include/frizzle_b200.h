@@ -451,6 +451,144 @@ fz_status fz_attention_static(const float *q, const void *key_cache, const void 
                               uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t window,
                               uint32_t position, uint32_t rows, float *out, void *stream);
 
+/* ------------------------------------------------------------------ paged cache
+ * A key/value cache in pages, for hosts that step sequences of different
+ * lengths and hand cache memory out a page at a time: no counterpart in the
+ * reference, whose sequences each own a ring (cache/kv.h).  The operators
+ * below are kernel-level: device memory the caller owns, work enqueued on
+ * `stream`, nothing allocated and nothing waited for, so every call can be
+ * captured into a graph and replayed with other lengths, tables and contents.
+ *
+ * Sequence s holds entries 0 .. lengths[s] - 1.  Entry j lies in slot
+ * j mod page_slots of pool page page_table[s * table_stride + j / page_slots];
+ * KV head h of slot i of page p starts at keys (values) + p page_stride +
+ * i slot_stride + h head_stride, in elements, head_dim elements in a row.  So
+ * slot-major and head-major pages are both only strides.  Slots past a
+ * sequence's length are never read, whatever they hold.  Pages that several
+ * sequences share may be read by all of them; fz_paged_append, weight
+ * accumulation and fz_paged_evict's `to` want pages of one sequence only.
+ *
+ * Lengths, tables and rows are device memory, so the host cannot check them:
+ * the kernels do.  What they find out of range is skipped, never followed,
+ * and, with `error` set, noted by OR-ing FZ_PAGED_BAD_* bits into that word:
+ * BAD_PAGE a held entry's table word that is no page of the pool (the entry is
+ * left out), BAD_LENGTH a length past the table (cut to it), BAD_ROW an
+ * appended row outside the sequences or the table (not stored), BAD_BLOCK a
+ * selected page that is not held, not above the word before it, or after a
+ * FZ_PAGED_NONE (left out; a list out of order may still name a page twice,
+ * and the call's results are then not to be used).  The caller zeroes the
+ * word. */
+typedef enum fz_kv_type { FZ_KV_F16 = 0, FZ_KV_BF16 = 1 } fz_kv_type;
+
+#define FZ_PAGED_BAD_PAGE 1u
+#define FZ_PAGED_BAD_LENGTH 2u
+#define FZ_PAGED_BAD_ROW 4u
+#define FZ_PAGED_BAD_BLOCK 8u
+#define FZ_PAGED_NONE 0xFFFFFFFFu
+
+typedef struct fz_paged_kv {
+  void *keys, *values;          /* 16-byte aligned */
+  const uint32_t *page_table;   /* [sequences][table_stride] */
+  uint32_t *lengths;            /* [sequences] entries held */
+  float *weights;               /* [pages][kv_heads][page_slots] accumulated attention weight, or NULL */
+  void *bounds;                 /* [pages][kv_heads][2][head_dim] least and greatest key, the cache's type, or NULL */
+  uint32_t *error;              /* one word, or NULL */
+  uint64_t page_stride, slot_stride, head_stride;  /* elements, multiples of 8 */
+  uint32_t sequences, table_stride, pages, page_slots, kv_heads;
+  uint32_t head_dim;            /* 64, 128 or 256 */
+  uint32_t type;                /* fz_kv_type */
+  uint32_t padding;
+} fz_paged_kv;
+
+/* Appended rows: row r is a token of sequence[r] (NULL: sequence r), stored as
+ * its entry index[r]; a row of sequence FZ_PAGED_NONE is padding and neither
+ * read nor written.  Each query and key head is normed over its head_dim
+ * values, x rsqrt(mean(x^2) + eps) gain (a NULL gain: not normed), then
+ * rotated by position[r] (NULL: index[r]): values i and i + head_dim / 2 by
+ * the angle 2 pi position turns[i], turns the frequencies in turns a position
+ * (NULL: not rotated; a pair with turns 0 stays).  The rotation is taken from
+ * the 64-bit product's fraction, so positions of any size keep f32 angles
+ * (rope.wgsl:120-138 reduces the f32 product).  Queries go to q_out as f32,
+ * which may be q itself; keys and values into the pages, rounded to nearest
+ * even, f16 saturating at +-65,504 (f16_pack.wgsl:16-19).  An appended entry's
+ * accumulated weight becomes 0, and lengths[s] grows to index + 1 where that
+ * is more.  Two rows of one call must not name the same entry. */
+typedef struct fz_paged_rows {
+  const float *q, *k, *v;       /* [rows][heads or kv_heads][head_dim], 16-byte aligned */
+  float *q_out;                 /* [rows][heads][head_dim] */
+  uint64_t q_stride, k_stride, v_stride, q_out_stride;  /* floats a row, multiples of 4 */
+  const float *q_gain, *k_gain; /* [head_dim] or NULL */
+  const double *turns;          /* [head_dim / 2] or NULL */
+  const uint32_t *sequence;     /* [rows] or NULL */
+  const uint32_t *index;        /* [rows] */
+  const uint32_t *position;     /* [rows] or NULL */
+  uint32_t rows;
+  uint32_t heads;               /* query heads, 0: keys and values only */
+  float eps;
+  uint32_t padding;
+} fz_paged_rows;
+fz_status fz_paged_append(const fz_paged_kv *kv, const fz_paged_rows *rows, void *stream);
+
+/* kv->bounds of every page that holds an entry of first[s] .. lengths[s] - 1
+ * (first NULL: every page held): over the page's held entries, each
+ * dimension's least and greatest key.  A NaN key makes its dimension's bounds
+ * NaN. */
+fz_status fz_paged_bounds(const fz_paged_kv *kv, const uint32_t *first, void *stream);
+
+/* The pages one query a sequence should attend to, a KV head at a time:
+ * blocks[s][h] = at most `top` logical pages of those sequence s holds, in
+ * ascending order, FZ_PAGED_NONE past them.  A page scores the largest value
+ * any of the KV head's query heads could reach in it, max over heads of
+ * sum_i max(q_i least_i, q_i greatest_i), in 64 bits; its first `sink` and
+ * last `recent` pages are taken first (sink + recent <= top), then the best
+ * scores, equal ones by the lower page, NaN before all numbers.  q as in
+ * fz_paged_attention.  scores: NULL or [sequences][kv_heads][top], each
+ * chosen page's score (0 past them).  Keys and values are not read. */
+fz_status fz_paged_select(const fz_paged_kv *kv, const float *q, uint64_t q_stride, uint32_t heads, uint32_t top,
+                          uint32_t sink, uint32_t recent, uint32_t *blocks, float *scores, void *stream);
+
+/* Attention of one new token a sequence: out[s] = softmax(scale q[s] . k_j) v_j
+ * over the entries j sequence s holds (the new token's own key appended
+ * first), with `window` the last `window` of them only, with `blocks` those in
+ * the selected pages only (as fz_paged_select leaves them: the first
+ * min(top, pages held) words of [sequences][kv_heads][top]).  1 to 8 query
+ * heads a KV head.  A sequence left with no entry, or only entries of weight
+ * zero, gives zeros.  With kv->weights, every entry that took part gets
+ * weights = decay weights + the sum of its softmax weights over the KV head's
+ * query heads (decay 0: the old value is not read).  workspace:
+ * fz_paged_attention_workspace bytes, 256-byte aligned, no initial value
+ * needed; calls that may overlap on the GPU must not share it. */
+typedef struct fz_paged_query {
+  const float *q;               /* [sequences][heads][head_dim], 16-byte aligned */
+  float *out;                   /* [sequences][heads][head_dim], 16-byte aligned */
+  uint64_t q_stride, out_stride;/* floats a sequence, multiples of 4 */
+  const uint32_t *blocks;       /* or NULL: every page */
+  void *workspace;
+  size_t workspace_bytes;
+  uint32_t heads;
+  uint32_t top;                 /* words a KV head in blocks */
+  uint32_t window;              /* 0: no window */
+  float scale;
+  float decay;
+  uint32_t padding;
+} fz_paged_query;
+fz_status fz_paged_attention(const fz_paged_kv *kv, const fz_paged_query *query, void *stream);
+/* Bytes of workspace for the cache as described (its weights pointer counts) and `heads` query heads. */
+size_t fz_paged_attention_workspace(const fz_paged_kv *kv, uint32_t heads);
+
+/* Keeps at most `budget` entries of each sequence and KV head and writes them,
+ * in order, into the other pages `to` describes (the same type and heads, its
+ * own table; none of them a page `from` holds): the first `sink` and the last
+ * `recent` entries first (sink + recent <= budget), then the largest
+ * accumulated weights, equal ones by the lower index, NaN before all numbers.
+ * Keys, values and weights are copied bit for bit, keys keeping the rotation
+ * of the position they were appended at; to->lengths[s] =
+ * min(from->lengths[s], budget), and kept[s][h] = the source index of each
+ * entry kept, FZ_PAGED_NONE past them ([sequences][kv_heads][budget]).  `from`
+ * is left as it was.  A window then counts kept entries. */
+fz_status fz_paged_evict(const fz_paged_kv *from, const fz_paged_kv *to, uint32_t budget, uint32_t sink,
+                         uint32_t recent, uint32_t *kept, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
