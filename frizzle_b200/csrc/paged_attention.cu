@@ -1,12 +1,19 @@
 // Attention of one new token a sequence over a paged cache (fz_paged_attention).
 #include "paged.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 namespace fz {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr uint32_t kCtas = 148;        // one an SM
+constexpr int kHalf = 8192;            // bytes of a tile's keys, and of its values
+constexpr int kSlots = 3;              // halves a warp holds
+constexpr int kMerge = 8192;           // floats the warps exchange their outputs through
+constexpr int kSmem = kWarps * kSlots * kHalf + kMerge * 4;
 
 struct AttendArgs {
   PagedView kv;
@@ -16,144 +23,669 @@ struct AttendArgs {
   const uint32_t* blocks;
   uint32_t group, top, window;
   float scale_log2e, decay;
+  uint32_t whole;          // items are never split
+  // Workspace.
+  float* part_o;           // [kCtas][2][group][D] unnormalised outputs of a CTA's first and last item
+  float2* part_ml;         // [kCtas][2][8] their maximum and sum
+  uint4* heads;            // [kCtas] the split item a CTA begins: {item, CTAs, its slot, 0}
+  float2* stats;           // [items][8] maximum and reciprocal sum, for the weights
+  float* scores;           // [items][score_stride][group] in log2 units, for the weights
+  uint64_t score_stride;
 };
 
-// Entry `i` of an item's list: its logical index, or FZ_PAGED_NONE.  Without
-// selected pages the list is the entries from `first` on.
-FZ_DEV uint32_t listed(const AttendArgs& a, const uint32_t* blocks, uint32_t i, uint32_t first, uint32_t n, bool say) {
+// A sequence's list: the entries a query attends to, `count` of them, without
+// selected pages those from `first` on, with them the pages' slots in order.
+struct List {
+  uint32_t n, first, count;
+};
+FZ_DEV List list_of(const AttendArgs& a, uint32_t s) {
+  List l;
+  l.n = held(a.kv, s);
+  l.first = a.window && l.n > a.window ? l.n - a.window : 0;
   const uint32_t slots = a.kv.page_slots;
-  if (!blocks) return first + i < n ? first + i : FZ_PAGED_NONE;
-  const uint32_t at = i / slots, b = __ldcg(blocks + at);
+  l.count = a.blocks ? min(a.top, (l.n + slots - 1) / slots) * slots : l.n - l.first;
+  return l;
+}
+
+// Entry i of an item's list: its logical index, or FZ_PAGED_NONE.
+FZ_DEV uint32_t listed(const AttendArgs& a, const uint32_t* blocks, uint32_t i, const List& l) {
+  if (i >= l.count) return FZ_PAGED_NONE;
+  if (!blocks) return l.first + i;
+  const uint32_t slots = a.kv.page_slots, at = i / slots, b = __ldcg(blocks + at);
   if (b == FZ_PAGED_NONE) return FZ_PAGED_NONE;
-  if (b >= (n + slots - 1) / slots || (at && __ldcg(blocks + at - 1) >= b)) {
-    if (say) note(a.kv, FZ_PAGED_BAD_BLOCK);
+  if (b >= (l.n + slots - 1) / slots || (at && __ldcg(blocks + at - 1) >= b)) {
+    note(a.kv, FZ_PAGED_BAD_BLOCK);
     return FZ_PAGED_NONE;
   }
   const uint32_t j = b * slots + i % slots;
-  return j < n && j >= first ? j : FZ_PAGED_NONE;
+  return j < l.n && j >= l.first ? j : FZ_PAGED_NONE;
 }
 
-// One CTA a (sequence, KV head), a warp an entry at a time with its own
-// running maximum and sum in log2 units, the warps joined at the end.
-template <class T, int D>
-__global__ void __launch_bounds__(32 * kWarps) attend_kernel(const AttendArgs a) {
-  constexpr int P = D / 64;
-  __shared__ float q[8 * D], o[8 * D], wm[kWarps][8], wl[kWarps][8];
-  pdl_wait();
-  const PagedView& v = a.kv;
-  const int G = a.group, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t h = blockIdx.x % v.kv_heads, s = blockIdx.x / v.kv_heads;
-  const uint32_t n = held(v, s);
-  if (threadIdx.x == 0 && h == 0 && __ldcg(v.lengths + s) > n) note(v, FZ_PAGED_BAD_LENGTH);
-  const uint32_t first = a.window && n > a.window ? n - a.window : 0;
-  const uint32_t* blocks = a.blocks ? a.blocks + (size_t)blockIdx.x * a.top : nullptr;
-  const uint32_t count = blocks ? min(a.top, (n + v.page_slots - 1) / v.page_slots) * v.page_slots : n - first;
-  for (int i = threadIdx.x; i < G * D; i += 32 * kWarps) {
-    q[i] = a.q[s * a.q_stride + (size_t)h * G * D + i] * a.scale_log2e;
-    o[i] = 0.f;
+// The page and slot of entry i of (s, h)'s list; false where there is none to read.
+FZ_DEV bool place(const AttendArgs& a, uint32_t s, uint32_t h, uint32_t i, const List& l, uint32_t& page, uint32_t& slot) {
+  const uint32_t* blocks = a.blocks ? a.blocks + ((size_t)s * a.kv.kv_heads + h) * a.top : nullptr;
+  const uint32_t j = listed(a, blocks, i, l);
+  if (j == FZ_PAGED_NONE) return false;
+  page = __ldcg(a.kv.table + (size_t)s * a.kv.table_stride + j / a.kv.page_slots);
+  slot = j % a.kv.page_slots;
+  if (page < a.kv.pages) return true;
+  note(a.kv, FZ_PAGED_BAD_PAGE);
+  return false;
+}
+
+// A CTA's share of all items' units (`unit` entries a unit), in order of
+// sequence and KV head: a contiguous run of ceil(all / CTAs) units, at least
+// `least`, so that every CTA reads as much as the others whatever the lengths.
+// Called by the whole block.
+struct Share {
+  uint32_t units;          // this CTA's
+  uint32_t s, h;           // the item of its first unit
+  uint32_t before;         // that item's units before it
+  uint64_t first, per;
+};
+FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit, uint32_t least) {
+  __shared__ uint64_t sum[kWarps];
+  __shared__ Share found;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const uint32_t S = a.kv.sequences, run = (S + kThreads - 1) / kThreads, s0 = min(S, t * run), s1 = min(S, s0 + run);
+  uint64_t mine = 0;
+  for (uint32_t s = s0; s < s1; s++) mine += (list_of(a, s).count + unit - 1) / unit;
+  uint64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
   }
+  if (lane == 31) sum[warp] = upto;
   __syncthreads();
-  float m[8], l[8], acc[8][2 * P];
-  for (int g = 0; g < 8; g++) {
-    m[g] = -INFINITY, l[g] = 0.f;
-    for (int c = 0; c < 2 * P; c++) acc[g][c] = 0.f;
-  }
-  auto score = [&](uint64_t at, int g) {
-    const uint32_t* k = reinterpret_cast<const uint32_t*>(v.keys + at);
-    float d = 0.f;
+  uint64_t all = 0, before = 0;
 #pragma unroll
-    for (int c = 0; c < P; c++) {
-      const float2 x = T::unpack(k[lane + 32 * c]), y = reinterpret_cast<const float2*>(q + g * D)[lane + 32 * c];
-      d = fmaf(x.x, y.x, fmaf(x.y, y.y, d));
-    }
-    return warp_sum(d);
-  };
-  auto place = [&](uint32_t i, uint32_t& page, uint32_t& slot) {
-    const uint32_t j = listed(a, blocks, i, first, n, lane == 0);
-    if (j == FZ_PAGED_NONE) return false;
-    page = __ldcg(v.table + (size_t)s * v.table_stride + j / v.page_slots), slot = j % v.page_slots;
-    if (page < v.pages) return true;
-    if (lane == 0) note(v, FZ_PAGED_BAD_PAGE);
-    return false;
-  };
-  for (uint32_t i = warp; i < count; i += kWarps) {
-    uint32_t page, slot;
-    if (!place(i, page, slot)) continue;
-    const uint64_t at = element(v, page, slot, h);
-    const uint32_t* val = reinterpret_cast<const uint32_t*>(v.values + at);
-#pragma unroll
-    for (int g = 0; g < 8; g++) {
-      if (g >= G) break;
-      const float d = score(at, g), mm = fmaxf(m[g], d), base = mm == -INFINITY ? 0.f : mm;
-      const float f = exp2f(m[g] - base), p = exp2f(d - base);
-      l[g] = fmaf(l[g], f, p);
-#pragma unroll
-      for (int c = 0; c < P; c++) {
-        const float2 x = T::unpack(val[lane + 32 * c]);
-        acc[g][2 * c] = fmaf(acc[g][2 * c], f, p * x.x);
-        acc[g][2 * c + 1] = fmaf(acc[g][2 * c + 1], f, p * x.y);
-      }
-      m[g] = mm;
-    }
-  }
-#pragma unroll
-  for (int g = 0; g < 8; g++)
-    if (lane == 0) wm[warp][g] = m[g], wl[warp][g] = l[g];
-  __syncthreads();
-  float top[8], sum[8];
-#pragma unroll
-  for (int g = 0; g < 8; g++) {
-    float mm = -INFINITY, ll = 0.f;
-    for (int w = 0; w < kWarps; w++) mm = fmaxf(mm, wm[w][g]);
-    top[g] = mm == -INFINITY ? 0.f : mm;
-    for (int w = 0; w < kWarps; w++) ll = fmaf(wl[w][g], exp2f(wm[w][g] - top[g]), ll);
-    sum[g] = ll;
-  }
   for (int w = 0; w < kWarps; w++) {
-    if (w == warp) {
+    if (w < warp) before += sum[w];
+    all += sum[w];
+  }
+  const uint64_t KV = a.kv.kv_heads;
+  all *= KV;
+  before = (before + upto - mine) * KV;
+  const uint64_t per = max((uint64_t)least, (all + gridDim.x - 1) / gridDim.x), first = blockIdx.x * per;
+  if (t == 0) found.units = 0;
+  __syncthreads();
+  if (first < all && before <= first && first < before + mine * KV) {
+    uint32_t s = s0;
+    for (;; s++) {
+      const uint64_t u = (list_of(a, s).count + unit - 1) / unit;
+      if (first < before + u * KV) {
+        found.h = (uint32_t)((first - before) / u);
+        found.before = (uint32_t)((first - before) % u);
+        break;
+      }
+      before += u * KV;
+    }
+    found.s = s;
+    found.units = (uint32_t)min(per, all - first);
+    found.first = first;
+    found.per = per;
+  }
+  __syncthreads();
+  return found;
+}
+
+// Walks a CTA's items that have entries: `at` is the item's first unit, counted
+// from the CTA's first (negative where an earlier CTA has some of it).
+struct Walk {
+  uint32_t s, h, units;
+  int at;
+  List l;
+};
+FZ_DEV void load(const AttendArgs& a, Walk& w, uint32_t unit) {
+  w.l = list_of(a, w.s);
+  w.units = (w.l.count + unit - 1) / unit;
+}
+// To the next item with entries; false past the last sequence.  Called by whole
+// warps, which look at 32 sequences at a time (a padded batch ends in many
+// empty ones).
+FZ_DEV bool next(const AttendArgs& a, Walk& w, uint32_t unit) {
+  w.at += (int)w.units;
+  if (++w.h < a.kv.kv_heads && w.units) return true;
+  w.h = 0;
+  w.units = 0;
+  for (uint32_t s = w.s + 1; s < a.kv.sequences; s += 32) {
+    const uint32_t mine = s + (threadIdx.x & 31);
+    const uint32_t some = __ballot_sync(0xffffffffu, mine < a.kv.sequences && list_of(a, mine).count != 0);
+    if (some) {
+      w.s = s + __ffs(some) - 1;
+      load(a, w, unit);
+      return true;
+    }
+  }
+  w.s = a.kv.sequences;
+  return false;
+}
+
+FZ_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+FZ_DEV void copy16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+FZ_DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+FZ_DEV void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+FZ_DEV void matrices(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+FZ_DEV void matrices_t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+FZ_DEV uint32_t transpose(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <class T>
+FZ_DEV void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (T::kType == FZ_KV_F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A pair of f32 as pairs of the cache's type that sum to it: f16 part and
+// remainder (22 bits), the remainder times `lift`; bf16 three parts (24 bits).
+template <class T>
+struct Parts {
+  static constexpr int N = T::kType == FZ_KV_F16 ? 2 : 3;
+  uint32_t w[4];
+};
+template <class T>
+FZ_DEV Parts<T> parts(float x, float y, float lift = 1.f) {
+  Parts<T> p;
 #pragma unroll
-      for (int g = 0; g < 8; g++) {
-        if (g >= G) break;
-        const float f = exp2f(m[g] - top[g]);
+  for (int i = 0; i < Parts<T>::N; i++) {
+    p.w[i] = T::pack(x, y);
+    const float2 u = T::unpack(p.w[i]);
+    x = (x - u.x) * lift, y = (y - u.y) * lift;
+  }
 #pragma unroll
-        for (int c = 0; c < P; c++) {
-          o[g * D + 2 * (lane + 32 * c)] += acc[g][2 * c] * f;
-          o[g * D + 2 * (lane + 32 * c) + 1] += acc[g][2 * c + 1] * f;
+  for (int i = Parts<T>::N; i < 4; i++) p.w[i] = 0;
+  return p;
+}
+
+// exp2 of a difference to the maximum of `m`'s side: 0 for a side without entries.
+FZ_DEV float fold(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
+
+// softmax(q k / sqrt d) v for one query a head over a paged list of entries.
+//
+// The products run on mma.sync m16n8k16 with the entries in the M axis and the
+// KV head's query heads in N: scores (16 keys x 8) += K (16 x 16) q^T, out^T
+// (16 dims x 8) += V^T p^T, so the cache is the A operand straight from shared
+// memory (ldmatrix, transposed for V) and nothing is padded but N.  f32
+// accuracy comes from the 8 columns: with 4 heads or fewer they hold the heads'
+// f16 parts and remainders side by side (GP = 4, one MMA a step for f16); with
+// more (GP = 8) one MMA a part.  q is scaled by a power of two a head, so its
+// parts keep 22 bits whatever its size, f16 weights by 2^15 and their remainders
+// by 2^11 more, so that many small ones still sum (to 2^-51 of the largest).  A tile's product starts from zero and is added to the
+// running output in f32 (the fold's multiply-add), so the tensor cores'
+// truncating accumulation never runs along the sequence.
+//
+// Bound by HBM: 2 x d x 2 bytes an entry, G x 4 flops a byte.  So each warp is a
+// stream of its own: it copies its tiles (8 KiB of keys, 8 of values: 4096 / d
+// entries) by 16-byte cp.async, swizzled against bank conflicts, into three
+// slots of 8 KiB, two in flight while one is used, 128 KiB in flight an SM, and
+// keeps its own running maximum, sum and output; no barrier until an item ends,
+// where the eight warps join in shared memory.  The copies run on into the next
+// item meanwhile.  Items are cut at equal shares of all entries; what a CTA has
+// of an item that others share goes to the workspace, and join_kernel adds
+// those up.
+template <class T, int D, int GP>
+__global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a) {
+  constexpr int KT = 4096 / D;                     // entries a tile
+  constexpr int MS = KT / 16;                      // 16-entry steps a tile
+  constexpr int KS = D / 16;                       // 16-dimension steps
+  constexpr int TERMS = Parts<T>::N;
+  constexpr int NT = (TERMS * GP + 7) / 8;         // column tiles
+  constexpr int CHAINS = 4 / MS;                   // independent sums a score
+  constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte pieces a row, rows a copy step
+  constexpr float kShift = T::kType == FZ_KV_F16 ? 15.f : 0.f;
+  constexpr float kLift = T::kType == FZ_KV_F16 ? 2048.f : 1.f;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ float2 ml[kWarps][8];
+  float* merge = reinterpret_cast<float*>(smem + kWarps * kSlots * kHalf);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t4 = lane & 3, g4 = lane >> 2;
+  const uint32_t ring = smem_u32(smem) + warp * kSlots * kHalf;
+  const PagedView& v = a.kv;
+  const uint32_t G = a.group, KV = v.kv_heads;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // This CTA's items: a share of the units, or whole items.
+  Walk seg{};
+  uint32_t units = 0xFFFFFFFFu, last_item = 0;     // units, or the item after the last
+  uint64_t first = 0, per = 1;
+  bool some;
+  if (a.whole) {
+    const uint64_t items = (uint64_t)v.sequences * KV;
+    const uint32_t i0 = (uint32_t)(items * blockIdx.x / gridDim.x);
+    last_item = (uint32_t)(items * (blockIdx.x + 1) / gridDim.x);
+    seg.s = i0 / KV, seg.h = i0 % KV;
+    some = i0 < last_item;
+    if (some) {
+      load(a, seg, KT);
+      if (!seg.units) some = next(a, seg, KT);
+    }
+  } else {
+    const Share sh = share_of(a, KT, kWarps);
+    units = sh.units;
+    some = units != 0;
+    first = sh.first, per = sh.per;
+    if (some) {
+      seg.s = sh.s, seg.h = sh.h;
+      load(a, seg, KT);
+      seg.at = -(int)sh.before;
+    }
+    if (threadIdx.x == 0) a.heads[blockIdx.x] = make_uint4(0, 0, 0, 0);
+  }
+  auto mine = [&](const Walk& w) { return a.whole ? w.s * KV + w.h < last_item : w.at < (int)units; };
+
+  // The copies' side: tile k of this warp is unit warp + 8 k of the CTA.
+  Walk ahead = seg;
+  bool more = some;
+  struct Where {
+    uint64_t off[(KT + 31) / 32];                  // this lane's rows, elements
+    uint64_t valid;                                // the tile's rows
+    bool any;                                      // a tile
+  };
+  int unit_ahead = warp;
+  auto find = [&]() {
+    Where w;
+    w.any = more && mine(ahead) && (a.whole || unit_ahead < (int)units);
+    while (w.any && unit_ahead >= ahead.at + (int)ahead.units) {
+      more = next(a, ahead, KT);
+      w.any = more && mine(ahead);
+    }
+    w.valid = 0;
+#pragma unroll
+    for (int c = 0; c < (KT + 31) / 32; c++) {
+      uint32_t page = 0, slot = 0;
+      const uint32_t row = lane + 32 * c;
+      const bool ok = w.any && row < KT &&
+                      place(a, ahead.s, ahead.h, (uint32_t)(unit_ahead - ahead.at) * KT + row, ahead.l, page, slot);
+      w.off[c] = ok ? element(v, page, slot, ahead.h) : 0;
+      w.valid |= (uint64_t)__ballot_sync(0xffffffffu, ok) << (32 * c);
+    }
+    unit_ahead += kWarps;
+    return w;
+  };
+  auto fetch = [&](const Where& w, const uint16_t* pool, int slot) {
+    if (w.any) {
+      const uint32_t base = ring + slot * kHalf;
+      const int piece = lane % CPR;
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int row = i * RPI + lane / CPR;
+        const uint64_t off = __shfl_sync(0xffffffffu, w.off[KT > 32 ? i / 8 : 0], row & 31);
+        copy16(base + row * (2 * D) + ((piece ^ (row & 7)) << 4), pool + off + piece * 8, (w.valid >> row) & 1);
+      }
+    }
+    copy_commit();
+  };
+  Where here = find(), soon = find();
+  fetch(here, v.keys, 0);
+  fetch(here, v.values, 1);
+  fetch(soon, v.keys, 2);
+  uint64_t valid = here.valid, valid_soon = soon.valid;
+  Where later = find();
+  int slot = 0;                                    // of the next half to use
+  int unit = warp;
+
+  while (some && mine(seg)) {
+    const int from = max(seg.at, 0), to = min(seg.at + (int)seg.units, (int)min(units, 0x7FFFFFFFu));
+    // q's parts as B operands, scaled so that each head's largest is in [1, 2).
+    uint32_t qf[KS][NT][2];
+    float c0, c1;                                  // the scores' factors of this lane's two columns' heads
+    {
+      const uint32_t g = g4 % GP;                  // the head of column g4 (all tiles)
+      const float* q = a.q + seg.s * a.q_stride + ((size_t)seg.h * G + min(g, G - 1)) * D + 2 * t4;
+      float2 x[KS][2];
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          x[k][i] = __ldcg(reinterpret_cast<const float2*>(q + 16 * k + 8 * i));
+          if (g >= G) x[k][i] = make_float2(0.f, 0.f);
+          top = fmaxf(top, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y)));
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);   // 2^(e - 127) <= top, normal and inverse normal
+      const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const Parts<T> p = parts<T>(x[k][i].x * down, x[k][i].y * down);
+#pragma unroll
+          for (int n = 0; n < NT; n++) qf[k][n][i] = GP == 8 ? p.w[n] : (g4 < 4 ? p.w[2 * n] : p.w[2 * n + 1]);
+        }
+      // Column g4's; this lane's columns are 2 t4 and 2 t4 + 1.  (An infinite q has no parts: NaN.)
+      const float c = top == INFINITY ? NAN : up * a.scale_log2e;
+      c0 = __shfl_sync(0xffffffffu, c, ((2 * t4) % GP) * 4);
+      c1 = __shfl_sync(0xffffffffu, c, ((2 * t4 + 1) % GP) * 4);
+    }
+    float o[KS][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[k][i] = 0.f;
+
+    for (; unit < to; unit += kWarps) {
+      // ---- scores
+      copy_wait<kSlots - 1>();
+      __syncwarp();
+      float s[MS][4];
+      {
+        float sc[MS][CHAINS][NT][4];
+#pragma unroll
+        for (int x = 0; x < MS * CHAINS * NT * 4; x++) (&sc[0][0][0][0])[x] = 0.f;
+        const uint32_t base = ring + slot * kHalf;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+          for (int ms = 0; ms < MS; ms++) {
+            uint32_t f[4];
+            const int row = ms * 16 + (lane & 15), piece = 2 * k + (lane >> 4);
+            matrices(f, base + row * (2 * D) + ((piece ^ (row & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; n++) mma<T>(sc[ms][k % CHAINS][n], f, qf[k][n][0], qf[k][n][1]);
+          }
+#pragma unroll
+        for (int ms = 0; ms < MS; ms++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            float x = 0.f;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+              for (int ch = 0; ch < CHAINS; ch++) x += sc[ms][ch][n][i];
+            if (GP == 4) x += __shfl_xor_sync(0xffffffffu, x, 2);
+            s[ms][i] = x;
+          }
+      }
+      __syncwarp();
+      fetch(soon, v.values, slot);
+      slot = slot == kSlots - 1 ? 0 : slot + 1;
+      float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+      for (int ms = 0; ms < MS; ms++) {
+        const bool lo = (valid >> (ms * 16 + g4)) & 1, hi = (valid >> (ms * 16 + g4 + 8)) & 1;
+        s[ms][0] = lo ? s[ms][0] * c0 : -INFINITY;
+        s[ms][1] = lo ? s[ms][1] * c1 : -INFINITY;
+        s[ms][2] = hi ? s[ms][2] * c0 : -INFINITY;
+        s[ms][3] = hi ? s[ms][3] * c1 : -INFINITY;
+        t0 = fmaxf(t0, fmaxf(s[ms][0], s[ms][2]));
+        t1 = fmaxf(t1, fmaxf(s[ms][1], s[ms][3]));
+      }
+      if (v.weights && 2 * t4 < GP) {
+        const uint64_t e = (seg.s * (uint64_t)KV + seg.h) * a.score_stride + (uint32_t)(unit - seg.at) * KT;
+#pragma unroll
+        for (int x = 0; x < 2 * MS; x++)
+#pragma unroll
+          for (int c = 0; c < 2; c++)
+            if ((valid >> (8 * x + g4)) & 1 && 2 * t4 + c < G)
+              a.scores[(e + 8 * x + g4) * G + 2 * t4 + c] = s[x / 2][2 * (x & 1) + c];
+      }
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, x));
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, x));
+      }
+      t0 = fmaxf(t0, m0), t1 = fmaxf(t1, m1);
+      const float b0 = t0 == -INFINITY ? 0.f : t0, b1 = t1 == -INFINITY ? 0.f : t1;
+      const float f0 = exp2f(m0 - b0), f1 = exp2f(m1 - b1);
+      m0 = t0, m1 = t1;
+      l0 *= f0, l1 *= f1;
+      uint32_t pf[MS][NT][2];
+#pragma unroll
+      for (int ms = 0; ms < MS; ms++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const float p0 = exp2f(s[ms][2 * i] - b0 + kShift), p1 = exp2f(s[ms][2 * i + 1] - b1 + kShift);
+          l0 += p0, l1 += p1;
+          const Parts<T> p = parts<T>(p0, p1, kLift);
+#pragma unroll
+          for (int n = 0; n < NT; n++) pf[ms][n][i] = transpose(GP == 8 ? p.w[n] : (t4 < 2 ? p.w[2 * n] : p.w[2 * n + 1]));
+        }
+      // ---- output
+      copy_wait<kSlots - 1>();
+      __syncwarp();
+      {
+        const uint32_t base = ring + slot * kHalf;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          float r[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ms = 0; ms < MS; ms++) {
+            uint32_t f[4];
+            const int row = ms * 16 + (lane & 7) + ((lane >> 4) << 3), piece = 2 * k + ((lane >> 3) & 1);
+            matrices_t(f, base + row * (2 * D) + ((piece ^ (row & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; n++) mma<T>(kLift > 1.f && n ? low : r, f, pf[ms][n][0], pf[ms][n][1]);
+          }
+          if (kLift > 1.f && GP == 8)
+#pragma unroll
+            for (int i = 0; i < 4; i++) r[i] = fmaf(low[i], 1.f / kLift, r[i]);
+          o[k][0] = fmaf(o[k][0], f0, r[0]);
+          o[k][1] = fmaf(o[k][1], f1, r[1]);
+          o[k][2] = fmaf(o[k][2], f0, r[2]);
+          o[k][3] = fmaf(o[k][3], f1, r[3]);
         }
       }
+      __syncwarp();
+      fetch(later, v.keys, slot);
+      slot = slot == kSlots - 1 ? 0 : slot + 1;
+      valid = valid_soon;
+      valid_soon = later.valid;
+      soon = later;
+      later = find();
     }
-    __syncthreads();
-  }
-  for (int i = threadIdx.x; i < G * D; i += 32 * kWarps) {
-    float l1 = 0.f;
+
+    // ---- the item's end: the warps' sums, maxima and outputs
 #pragma unroll
-    for (int g = 0; g < 8; g++) l1 = i / D == g ? sum[g] : l1;
-    a.out[s * a.out_stride + (size_t)h * G * D + i] = l1 == 0.f ? 0.f : o[i] / l1;
+    for (int x = 4; x < 32; x <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+    }
+    if (g4 == 0 && 2 * t4 < GP) ml[warp][2 * t4] = make_float2(m0, l0), ml[warp][2 * t4 + 1] = make_float2(m1, l1);
+    if (GP == 4) {
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float x = t4 < 2 ? o[k][i] : o[k][i] * (1.f / kLift);
+          o[k][i] = x + __shfl_xor_sync(0xffffffffu, x, 2);
+        }
+    }
+    const bool is_whole = seg.at >= 0 && seg.at + (int)seg.units == to;
+    const uint32_t part = blockIdx.x * 2 + (from > 0 ? 1 : 0);
+    const uint64_t item = seg.s * (uint64_t)KV + seg.h;
+    constexpr int DR = D * GP > 1024 ? 1024 / GP : D;    // dimensions a round
+#pragma unroll
+    for (int r = 0; r < D / DR; r++) {
+      if (2 * t4 < GP) {
+#pragma unroll
+        for (int k = 0; k < DR / 16; k++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            merge[(warp * GP + 2 * t4 + (i & 1)) * DR + 16 * k + g4 + 8 * (i >> 1)] = o[r * (DR / 16) + k][i];
+      }
+      __syncthreads();
+      const uint32_t g = threadIdx.x / (DR / 4), d = threadIdx.x % (DR / 4) * 4;
+      if (g < G) {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) top = fmaxf(top, ml[w][g].x);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+          const float2 y = ml[w][g];
+          const float f = fold(y.x, top);
+          const float4 z = *reinterpret_cast<const float4*>(merge + (w * GP + g) * DR + d);
+          sum = fmaf(y.y, f, sum);
+          x.x = fmaf(z.x, f, x.x), x.y = fmaf(z.y, f, x.y), x.z = fmaf(z.z, f, x.z), x.w = fmaf(z.w, f, x.w);
+        }
+        if (is_whole) {
+          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+          *reinterpret_cast<float4*>(a.out + seg.s * a.out_stride + (seg.h * (size_t)G + g) * D + r * DR + d) =
+              make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+          if (v.weights && r == 0 && d == 0) a.stats[item * 8 + g] = make_float2(sum == 0.f ? 0.f : top - kShift, inv);
+        } else {
+          *reinterpret_cast<float4*>(a.part_o + ((size_t)part * G + g) * D + r * DR + d) = x;
+          if (r == 0 && d == 0) a.part_ml[part * 8 + g] = make_float2(top, sum);
+        }
+      }
+      __syncthreads();
+    }
+    if (!is_whole && seg.at >= 0 && threadIdx.x == 0) {
+      const uint64_t end = first + (uint64_t)(seg.at + (int64_t)seg.units) - 1;
+      a.heads[blockIdx.x] = make_uint4((uint32_t)item, (uint32_t)(end / per) - blockIdx.x + 1, from > 0 ? 1u : 0u, 0u);
+    }
+    some = next(a, seg, KT);
   }
-  if (!v.weights) return;
-  for (uint32_t i = warp; i < count; i += kWarps) {
+  copy_wait<0>();
+
+  // Sequences without entries: zeros, a warp a sequence.
+  for (uint32_t s0 = (blockIdx.x * kWarps + warp) * 32; s0 < v.sequences; s0 += gridDim.x * kThreads) {
+    const uint32_t s = s0 + lane;
+    bool empty = false;
+    if (s < v.sequences) {
+      const List l = list_of(a, s);
+      if (__ldcg(v.lengths + s) > l.n) note(v, FZ_PAGED_BAD_LENGTH);
+      empty = l.count == 0;
+    }
+    for (uint32_t left = __ballot_sync(0xffffffffu, empty); left; left &= left - 1) {
+      float4* out = reinterpret_cast<float4*>(a.out + (s0 + __ffs(left) - 1) * a.out_stride);
+      for (uint32_t i = lane; i < KV * G * D / 4; i += 32) out[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+}
+
+// The outputs of items that several CTAs share: CTA (c, g) adds up head g of
+// the item CTA c begins, from parts in order, so the sum never depends on who
+// came first.
+template <int D, bool F16>
+__global__ void __launch_bounds__(kThreads) join_kernel(const AttendArgs a) {
+  constexpr int COLS = D / 4, LANES = kThreads / COLS;
+  __shared__ float2 ml[kCtas];
+  __shared__ float4 sums[kThreads];
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint4 h = __ldcg(a.heads + blockIdx.x);
+  const uint32_t parts = h.y, g = blockIdx.y;
+  if (!parts) return;
+  auto part = [&](uint32_t i) { return (blockIdx.x + i) * 2 + (i == 0 ? h.z : 0u); };
+  for (uint32_t i = threadIdx.x; i < parts; i += kThreads) ml[i] = __ldcg(a.part_ml + part(i) * 8 + g);
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f;
+  for (uint32_t i = 0; i < parts; i++) top = fmaxf(top, ml[i].x);
+  for (uint32_t i = 0; i < parts; i++) sum = fmaf(ml[i].y, fold(ml[i].x, top), sum);
+  const int col = threadIdx.x % COLS;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (uint32_t i = threadIdx.x / COLS; i < parts; i += LANES) {
+    const float4 z = __ldcg(reinterpret_cast<const float4*>(a.part_o + ((size_t)part(i) * a.group + g) * D) + col);
+    const float f = fold(ml[i].x, top);
+    x.x = fmaf(z.x, f, x.x), x.y = fmaf(z.y, f, x.y), x.z = fmaf(z.z, f, x.z), x.w = fmaf(z.w, f, x.w);
+  }
+  sums[threadIdx.x] = x;
+  __syncthreads();
+  if (threadIdx.x >= COLS) return;
+#pragma unroll
+  for (int i = 1; i < LANES; i++) {
+    const float4 z = sums[i * COLS + col];
+    x.x += z.x, x.y += z.y, x.z += z.z, x.w += z.w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const uint32_t s = h.x / a.kv.kv_heads, kvh = h.x % a.kv.kv_heads;
+  *reinterpret_cast<float4*>(a.out + s * a.out_stride + (kvh * (size_t)a.group + g) * D + 4 * col) =
+      make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  if (a.kv.weights && col == 0) a.stats[(size_t)h.x * 8 + g] = make_float2(sum == 0.f ? 0.f : top - (F16 ? 15.f : 0.f), inv);
+}
+
+// The entries' weights from the scores and the items' maxima and sums, 32
+// entries a warp at a time, each entry written by the one lane it falls to.
+__global__ void __launch_bounds__(kThreads) weigh_kernel(const AttendArgs a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const Share sh = share_of(a, 32, kWarps);
+  if (!sh.units) return;
+  const int lane = threadIdx.x & 31;
+  const PagedView& v = a.kv;
+  Walk w{};
+  w.s = sh.s, w.h = sh.h;
+  load(a, w, 32);
+  w.at = -(int)sh.before;
+  for (int u = threadIdx.x >> 5; u < (int)sh.units; u += kWarps) {
+    bool more = true;
+    while (more && u >= w.at + (int)w.units) more = next(a, w, 32);
+    if (!more) return;
+    const uint32_t i = (uint32_t)(u - w.at) * 32 + lane;
     uint32_t page, slot;
-    if (!place(i, page, slot)) continue;
-    const uint64_t at = element(v, page, slot, h);
-    float w = 0.f;
-#pragma unroll
-    for (int g = 0; g < 8; g++) {
-      if (g >= G) break;
-      const float p = exp2f(score(at, g) - top[g]);
-      w += sum[g] == 0.f ? 0.f : p / sum[g];
+    if (place(a, w.s, w.h, i, w.l, page, slot)) {
+      const uint64_t item = w.s * (uint64_t)v.kv_heads + w.h;
+      float sum = 0.f;
+      for (uint32_t g = 0; g < a.group; g++) {
+        const float2 st = __ldcg(a.stats + item * 8 + g);
+        sum = fmaf(exp2f(__ldcg(a.scores + (item * a.score_stride + i) * a.group + g) - st.x), st.y, sum);
+      }
+      float* to = v.weights + ((size_t)page * v.kv_heads + w.h) * v.page_slots + slot;
+      *to = a.decay == 0.f ? sum : fmaf(a.decay, *to, sum);
     }
-    float* to = v.weights + ((size_t)page * v.kv_heads + h) * v.page_slots + slot;
-    if (lane == 0) *to = a.decay == 0.f ? w : fmaf(a.decay, *to, w);
+    __syncwarp();
   }
+}
+
+template <class T, int D>
+const void* attend_of(uint32_t group) {
+  return group <= 4 ? (const void*)attend_kernel<T, D, 4> : (const void*)attend_kernel<T, D, 8>;
+}
+template <class T>
+const void* attend_of(uint32_t d, uint32_t group) {
+  return d == 64 ? attend_of<T, 64>(group) : d == 128 ? attend_of<T, 128>(group) : attend_of<T, 256>(group);
+}
+template <bool F16>
+const void* join_of(uint32_t d) {
+  return d == 64    ? (const void*)join_kernel<64, F16>
+         : d == 128 ? (const void*)join_kernel<128, F16>
+                    : (const void*)join_kernel<256, F16>;
+}
+
+// Where each part of the workspace begins; returns its whole size.
+size_t layout(const fz_paged_kv* kv, uint32_t heads, size_t (&at)[5]) {
+  const uint64_t group = heads / std::max(1u, kv->kv_heads), items = (uint64_t)kv->sequences * kv->kv_heads;
+  const uint64_t entries = (uint64_t)kv->table_stride * kv->page_slots;
+  const uint64_t bytes[5] = {kCtas * 2ull * group * kv->head_dim * 4, kCtas * 2ull * 8 * 8, kCtas * 16ull,
+                             kv->weights ? items * 64 : 0, kv->weights ? items * entries * group * 4 : 0};
+  size_t end = 0;
+  for (int i = 0; i < 5; i++) {
+    at[i] = end;
+    end += (bytes[i] + 255) / 256 * 256;
+  }
+  return end;
 }
 
 }  // namespace
 }  // namespace fz
 
 extern "C" size_t fz_paged_attention_workspace(const fz_paged_kv* kv, uint32_t heads) {
-  (void)kv;
-  (void)heads;
-  return 256;
+  size_t at[5];
+  return kv ? fz::layout(kv, heads, at) : 0;
 }
 
 extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_query* query, void* stream) {
@@ -190,14 +722,38 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   a.blocks = query->blocks, a.group = heads / kv->kv_heads, a.top = query->top, a.window = query->window;
   a.scale_log2e = (float)((double)query->scale * 1.4426950408889634);
   a.decay = query->decay;
+  size_t at[5];
+  layout(kv, heads, at);
+  char* w = static_cast<char*>(query->workspace);
+  a.part_o = reinterpret_cast<float*>(w + at[0]);
+  a.part_ml = reinterpret_cast<float2*>(w + at[1]);
+  a.heads = reinterpret_cast<uint4*>(w + at[2]);
+  a.stats = reinterpret_cast<float2*>(w + at[3]);
+  a.scores = reinterpret_cast<float*>(w + at[4]);
+  a.score_stride = (uint64_t)kv->table_stride * kv->page_slots;
+  // The longest list an item can have, in tiles: with at most one a warp,
+  // items stay whole (no join, and no CTA needs every length).
+  uint64_t most = a.score_stride;
+  if (a.blocks) most = std::min<uint64_t>(most, (uint64_t)a.top * kv->page_slots);
+  else if (a.window) most = std::min<uint64_t>(most, a.window);
+  const uint32_t tile = 4096 / kv->head_dim;
+  const uint64_t tiles = (most + tile - 1) / tile;
+  a.whole = tiles <= kWarps;
+  const uint32_t grid =
+      (uint32_t)std::min<uint64_t>(kCtas, a.whole ? items : (items * tiles + kWarps - 1) / kWarps);
   void* args[] = {&a};
   const bool f16 = kv->type == FZ_KV_F16;
   const uint32_t d = kv->head_dim;
-  const void* fn = f16 ? (d == 64    ? (const void*)attend_kernel<F16, 64>
-                          : d == 128 ? (const void*)attend_kernel<F16, 128>
-                                     : (const void*)attend_kernel<F16, 256>)
-                       : (d == 64    ? (const void*)attend_kernel<Bf16, 64>
-                          : d == 128 ? (const void*)attend_kernel<Bf16, 128>
-                                     : (const void*)attend_kernel<Bf16, 256>);
-  return paged_launch(fn, dim3((uint32_t)items), dim3(32 * kWarps), 0, 1, args, stream);
+  if ((st = paged_launch(f16 ? attend_of<F16>(d, a.group) : attend_of<Bf16>(d, a.group), dim3(grid), dim3(kThreads), kSmem, 1,
+                         args, stream)))
+    return st;
+  if (!a.whole &&
+      (st = paged_launch(f16 ? join_of<true>(d) : join_of<false>(d), dim3(grid, a.group), dim3(kThreads), 0, 1, args, stream)))
+    return st;
+  if (a.kv.weights) {
+    const uint64_t units = items * ((most + 31) / 32);
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>(4 * kCtas, (units + kWarps - 1) / kWarps);
+    st = paged_launch((const void*)weigh_kernel, dim3(blocks), dim3(kThreads), 0, 1, args, stream);
+  }
+  return st;
 }
