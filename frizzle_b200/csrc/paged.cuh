@@ -50,7 +50,7 @@ FZ_DEV void note(const PagedView& v, uint32_t bit) {
 
 // Entries sequence s holds, cut to its table.
 FZ_DEV uint32_t held(const PagedView& v, uint32_t s) {
-  const uint32_t n = __ldcg(v.lengths + s);
+  const uint32_t n = v.lengths[s];
   return min(n, v.table_stride * v.page_slots);
 }
 

@@ -28,7 +28,8 @@ struct AttendArgs {
   float* part_o;           // [kCtas][2][group][D] unnormalised outputs of a CTA's first and last item
   float2* part_ml;         // [kCtas][2][8] their maximum and sum
   uint4* heads;            // [kCtas] the split item a CTA begins: {item, CTAs, its slot, 0}
-  float2* stats;           // [items][8] maximum and reciprocal sum, for the weights
+  uint4* origin;           // [items] where an item's outputs are, for the weights: {first CTA, CTAs, its slot, 0}
+  float2* stats;           // [items][8] an unsplit item's maximum and reciprocal sum, for the weights
   float* scores;           // [items][score_stride][group] in log2 units, for the weights
   uint64_t score_stride;
 };
@@ -51,9 +52,9 @@ FZ_DEV List list_of(const AttendArgs& a, uint32_t s) {
 FZ_DEV uint32_t listed(const AttendArgs& a, const uint32_t* blocks, uint32_t i, const List& l) {
   if (i >= l.count) return FZ_PAGED_NONE;
   if (!blocks) return l.first + i;
-  const uint32_t slots = a.kv.page_slots, at = i / slots, b = __ldcg(blocks + at);
+  const uint32_t slots = a.kv.page_slots, at = i / slots, b = blocks[at];
   if (b == FZ_PAGED_NONE) return FZ_PAGED_NONE;
-  if (b >= (l.n + slots - 1) / slots || (at && __ldcg(blocks + at - 1) >= b)) {
+  if (b >= (l.n + slots - 1) / slots || (at && blocks[at - 1] >= b)) {
     note(a.kv, FZ_PAGED_BAD_BLOCK);
     return FZ_PAGED_NONE;
   }
@@ -66,30 +67,36 @@ FZ_DEV bool place(const AttendArgs& a, uint32_t s, uint32_t h, uint32_t i, const
   const uint32_t* blocks = a.blocks ? a.blocks + ((size_t)s * a.kv.kv_heads + h) * a.top : nullptr;
   const uint32_t j = listed(a, blocks, i, l);
   if (j == FZ_PAGED_NONE) return false;
-  page = __ldcg(a.kv.table + (size_t)s * a.kv.table_stride + j / a.kv.page_slots);
+  page = a.kv.table[(size_t)s * a.kv.table_stride + j / a.kv.page_slots];
   slot = j % a.kv.page_slots;
   if (page < a.kv.pages) return true;
   note(a.kv, FZ_PAGED_BAD_PAGE);
   return false;
 }
 
-// A CTA's share of all items' units (`unit` entries a unit), in order of
-// sequence and KV head: a contiguous run of ceil(all / CTAs) units, at least
-// `least`, so that every CTA reads as much as the others whatever the lengths.
-// Called by the whole block.
+// CTA `cta` of `ctas`' share of all items' units (`unit` entries a unit, and
+// before each item `extra` that stand for what beginning an item costs), in
+// order of sequence and KV head: a contiguous run of ceil(all / ctas) units, at
+// least `least`, so that every CTA takes as long as the others whatever the
+// lengths.  Called by the whole block.
 struct Share {
   uint32_t units;          // this CTA's
   uint32_t s, h;           // the item of its first unit
-  uint32_t before;         // that item's units before it
+  int at;                  // where that item's entries begin, from the CTA's first unit
+  List l;                  // its list
   uint64_t first, per;
 };
-FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit, uint32_t least) {
+FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit, uint32_t extra, uint32_t least, uint32_t cta, uint32_t ctas) {
   __shared__ uint64_t sum[kWarps];
   __shared__ Share found;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const uint32_t S = a.kv.sequences, run = (S + kThreads - 1) / kThreads, s0 = min(S, t * run), s1 = min(S, s0 + run);
   uint64_t mine = 0;
-  for (uint32_t s = s0; s < s1; s++) mine += (list_of(a, s).count + unit - 1) / unit;
+  List l{};
+  for (uint32_t s = s0; s < s1; s++) {
+    l = list_of(a, s);
+    if (l.count) mine += (l.count + unit - 1) / unit + extra;
+  }
   uint64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -97,6 +104,7 @@ FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit, uint32_t least) {
     if (lane >= o) upto += x;
   }
   if (lane == 31) sum[warp] = upto;
+  if (t == 0) found.units = 0;
   __syncthreads();
   uint64_t all = 0, before = 0;
 #pragma unroll
@@ -107,20 +115,20 @@ FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit, uint32_t least) {
   const uint64_t KV = a.kv.kv_heads;
   all *= KV;
   before = (before + upto - mine) * KV;
-  const uint64_t per = max((uint64_t)least, (all + gridDim.x - 1) / gridDim.x), first = blockIdx.x * per;
-  if (t == 0) found.units = 0;
-  __syncthreads();
+  const uint64_t even = (all >> 32) ? (all + ctas - 1) / ctas : ((uint32_t)all + (ctas - 1)) / ctas;
+  const uint64_t per = max((uint64_t)least, even), first = cta * per;
   if (first < all && before <= first && first < before + mine * KV) {
-    uint32_t s = s0;
+    uint32_t s = s0, u;
     for (;; s++) {
-      const uint64_t u = (list_of(a, s).count + unit - 1) / unit;
-      if (first < before + u * KV) {
-        found.h = (uint32_t)((first - before) / u);
-        found.before = (uint32_t)((first - before) % u);
-        break;
-      }
+      if (run > 1) l = list_of(a, s);
+      u = l.count ? (l.count + unit - 1) / unit + extra : 0u;
+      if (first < before + u * KV) break;
       before += u * KV;
     }
+    const uint64_t in = first - before;
+    found.h = KV == 1 ? 0u : (uint32_t)(in / u);
+    found.at = (int)(extra + (int64_t)found.h * u - (int64_t)in);
+    found.l = l;
     found.s = s;
     found.units = (uint32_t)min(per, all - first);
     found.first = first;
@@ -144,8 +152,8 @@ FZ_DEV void load(const AttendArgs& a, Walk& w, uint32_t unit) {
 // To the next item with entries; false past the last sequence.  Called by whole
 // warps, which look at 32 sequences at a time (a padded batch ends in many
 // empty ones).
-FZ_DEV bool next(const AttendArgs& a, Walk& w, uint32_t unit) {
-  w.at += (int)w.units;
+FZ_DEV bool next(const AttendArgs& a, Walk& w, uint32_t unit, uint32_t extra) {
+  w.at += (int)(w.units + extra);
   if (++w.h < a.kv.kv_heads && w.units) return true;
   w.h = 0;
   w.units = 0;
@@ -160,6 +168,11 @@ FZ_DEV bool next(const AttendArgs& a, Walk& w, uint32_t unit) {
   }
   w.s = a.kv.sequences;
   return false;
+}
+
+// The item a share begins with.
+FZ_DEV Walk begin(const Share& sh, uint32_t unit) {
+  return Walk{sh.s, sh.h, (sh.l.count + unit - 1) / unit, sh.at, sh.l};
 }
 
 FZ_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -256,7 +269,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   constexpr float kLift = T::kType == FZ_KV_F16 ? 2048.f : 1.f;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ float2 ml[kWarps][8];
+  __shared__ float qc[8];                          // the scores' factor of each head
+  // The warps' exchange at an item's end; until then q's B operands.
   float* merge = reinterpret_cast<float*>(smem + kWarps * kSlots * kHalf);
+  uint2* qf = reinterpret_cast<uint2*>(merge);     // [KS][NT][32], 12 KiB at most
+  float4* raw = reinterpret_cast<float4*>(merge + 4096);   // [GP][D / 4]
+  __shared__ float largest[16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t4 = lane & 3, g4 = lane >> 2;
   const uint32_t ring = smem_u32(smem) + warp * kSlots * kHalf;
   const PagedView& v = a.kv;
@@ -277,21 +295,71 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
     some = i0 < last_item;
     if (some) {
       load(a, seg, KT);
-      if (!seg.units) some = next(a, seg, KT);
+      if (!seg.units) {
+        some = next(a, seg, KT, kWarps);
+        seg.at = 0;
+      }
     }
   } else {
-    const Share sh = share_of(a, KT, kWarps);
+    const Share sh = share_of(a, KT, kWarps, 2 * kWarps, blockIdx.x, gridDim.x);
     units = sh.units;
     some = units != 0;
     first = sh.first, per = sh.per;
-    if (some) {
-      seg.s = sh.s, seg.h = sh.h;
-      load(a, seg, KT);
-      seg.at = -(int)sh.before;
-    }
+    if (some) seg = begin(sh, KT);
     if (threadIdx.x == 0) a.heads[blockIdx.x] = make_uint4(0, 0, 0, 0);
   }
   auto mine = [&](const Walk& w) { return a.whole ? w.s * KV + w.h < last_item : w.at < (int)units; };
+
+  // An item's q, a few floats a thread, asked for an item ahead: a load waits
+  // behind all the copies in flight, some 3 us.
+  constexpr int QV = (GP * D + 4 * kThreads - 1) / (4 * kThreads);
+  float4 q_next[QV];
+  auto ask_q = [&](const Walk& w) {
+    const float4* q = reinterpret_cast<const float4*>(a.q + w.s * a.q_stride + (size_t)w.h * G * D);
+#pragma unroll
+    for (int r = 0; r < QV; r++) {
+      const int f = threadIdx.x + r * kThreads;
+      q_next[r] = f < (int)(G * D / 4) ? __ldcg(q + f) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  // Its parts as B operands in shared memory, scaled so that each head's largest
+  // is in [1, 2).
+  auto put_q = [&]() {
+    constexpr int W = D / 4 < 32 ? D / 4 : 32, PER = D / 4 / W;     // lanes a group, groups a head
+#pragma unroll
+    for (int r = 0; r < QV; r++) {
+      const int f = threadIdx.x + r * kThreads;
+      const float4 x = q_next[r];
+      float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+#pragma unroll
+      for (int o = W / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (f < GP * D / 4) {
+        raw[f] = x;
+        if (f % W == 0) largest[f / W] = top;
+      }
+    }
+    __syncthreads();
+    const int g = g4 % GP;                         // the head of column g4 (all tiles)
+    float top = largest[g * PER];
+#pragma unroll
+    for (int i = 1; i < PER; i++) top = fmaxf(top, largest[g * PER + i]);
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);   // 2^(e - 127) <= top, normal and inverse normal
+    const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
+    const float2* q = reinterpret_cast<const float2*>(raw) + g * (D / 2) + t4;
+    for (int k = warp; k < KS; k += kWarps) {
+      const float2 x = q[8 * k], y = q[8 * k + 4];
+      const Parts<T> p0 = parts<T>(x.x * down, x.y * down), p1 = parts<T>(y.x * down, y.y * down);
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+        qf[(k * NT + n) * 32 + lane] = GP == 8 ? make_uint2(p0.w[n], p1.w[n])
+                                               : (g4 < 4 ? make_uint2(p0.w[2 * n], p1.w[2 * n])
+                                                         : make_uint2(p0.w[2 * n + 1], p1.w[2 * n + 1]));
+    }
+    // (An infinite q has no parts: NaN.)
+    if (warp == 0 && t4 == 0 && g4 < GP) qc[g4] = top == INFINITY ? NAN : up * a.scale_log2e;
+    __syncthreads();
+  };
+  if (some) ask_q(seg);                            // (before the copies)
 
   // The copies' side: tile k of this warp is unit warp + 8 k of the CTA.
   Walk ahead = seg;
@@ -304,10 +372,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   int unit_ahead = warp;
   auto find = [&]() {
     Where w;
-    w.any = more && mine(ahead) && (a.whole || unit_ahead < (int)units);
-    while (w.any && unit_ahead >= ahead.at + (int)ahead.units) {
-      more = next(a, ahead, KT);
-      w.any = more && mine(ahead);
+    w.any = more;
+    while (w.any) {
+      // (The units before an item's first hold nothing.)
+      if (unit_ahead < ahead.at) unit_ahead += (ahead.at - unit_ahead + kWarps - 1) / kWarps * kWarps;
+      w.any = mine(ahead) && (a.whole || unit_ahead < (int)units);
+      if (!w.any || unit_ahead < ahead.at + (int)ahead.units) break;
+      w.any = more = next(a, ahead, KT, kWarps);
     }
     w.valid = 0;
 #pragma unroll
@@ -346,39 +417,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
 
   while (some && mine(seg)) {
     const int from = max(seg.at, 0), to = min(seg.at + (int)seg.units, (int)min(units, 0x7FFFFFFFu));
-    // q's parts as B operands, scaled so that each head's largest is in [1, 2).
-    uint32_t qf[KS][NT][2];
-    float c0, c1;                                  // the scores' factors of this lane's two columns' heads
-    {
-      const uint32_t g = g4 % GP;                  // the head of column g4 (all tiles)
-      const float* q = a.q + seg.s * a.q_stride + ((size_t)seg.h * G + min(g, G - 1)) * D + 2 * t4;
-      float2 x[KS][2];
-      float top = 0.f;
-#pragma unroll
-      for (int k = 0; k < KS; k++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          x[k][i] = __ldcg(reinterpret_cast<const float2*>(q + 16 * k + 8 * i));
-          if (g >= G) x[k][i] = make_float2(0.f, 0.f);
-          top = fmaxf(top, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y)));
-        }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);   // 2^(e - 127) <= top, normal and inverse normal
-      const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
-#pragma unroll
-      for (int k = 0; k < KS; k++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const Parts<T> p = parts<T>(x[k][i].x * down, x[k][i].y * down);
-#pragma unroll
-          for (int n = 0; n < NT; n++) qf[k][n][i] = GP == 8 ? p.w[n] : (g4 < 4 ? p.w[2 * n] : p.w[2 * n + 1]);
-        }
-      // Column g4's; this lane's columns are 2 t4 and 2 t4 + 1.  (An infinite q has no parts: NaN.)
-      const float c = top == INFINITY ? NAN : up * a.scale_log2e;
-      c0 = __shfl_sync(0xffffffffu, c, ((2 * t4) % GP) * 4);
-      c1 = __shfl_sync(0xffffffffu, c, ((2 * t4 + 1) % GP) * 4);
-    }
+    if (unit < seg.at) unit += (seg.at - unit + kWarps - 1) / kWarps * kWarps;
+    put_q();
+    Walk after = seg;
+    const bool then = next(a, after, KT, kWarps);
+    if (then && mine(after)) ask_q(after);
+    const float c0 = qc[(2 * t4) % GP], c1 = qc[(2 * t4 + 1) % GP];
     float o[KS][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
     for (int k = 0; k < KS; k++)
@@ -396,15 +440,19 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
         for (int x = 0; x < MS * CHAINS * NT * 4; x++) (&sc[0][0][0][0])[x] = 0.f;
         const uint32_t base = ring + slot * kHalf;
 #pragma unroll
-        for (int k = 0; k < KS; k++)
+        for (int k = 0; k < KS; k++) {
+          uint2 b[NT];
+#pragma unroll
+          for (int n = 0; n < NT; n++) b[n] = qf[(k * NT + n) * 32 + lane];
 #pragma unroll
           for (int ms = 0; ms < MS; ms++) {
             uint32_t f[4];
             const int row = ms * 16 + (lane & 15), piece = 2 * k + (lane >> 4);
             matrices(f, base + row * (2 * D) + ((piece ^ (row & 7)) << 4));
 #pragma unroll
-            for (int n = 0; n < NT; n++) mma<T>(sc[ms][k % CHAINS][n], f, qf[k][n][0], qf[k][n][1]);
+            for (int n = 0; n < NT; n++) mma<T>(sc[ms][k % CHAINS][n], f, b[n].x, b[n].y);
           }
+        }
 #pragma unroll
         for (int ms = 0; ms < MS; ms++)
 #pragma unroll
@@ -515,6 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
     const bool is_whole = seg.at >= 0 && seg.at + (int)seg.units == to;
     const uint32_t part = blockIdx.x * 2 + (from > 0 ? 1 : 0);
     const uint64_t item = seg.s * (uint64_t)KV + seg.h;
+    __syncthreads();                               // (every warp is done with q's operands)
     constexpr int DR = D * GP > 1024 ? 1024 / GP : D;    // dimensions a round
 #pragma unroll
     for (int r = 0; r < D / DR; r++) {
@@ -552,11 +601,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
       }
       __syncthreads();
     }
-    if (!is_whole && seg.at >= 0 && threadIdx.x == 0) {
+    if (seg.at >= 0 && threadIdx.x == 0) {
       const uint64_t end = first + (uint64_t)(seg.at + (int64_t)seg.units) - 1;
-      a.heads[blockIdx.x] = make_uint4((uint32_t)item, (uint32_t)(end / per) - blockIdx.x + 1, from > 0 ? 1u : 0u, 0u);
+      const uint32_t ctas = is_whole ? 0u : (uint32_t)(end / per) - blockIdx.x + 1;
+      if (!is_whole) a.heads[blockIdx.x] = make_uint4((uint32_t)item, ctas, from > 0 ? 1u : 0u, 0u);
+      if (v.weights) a.origin[item] = make_uint4(blockIdx.x, ctas, from > 0 ? 1u : 0u, 0u);
     }
-    some = next(a, seg, KT);
+    seg = after;
+    some = then;
   }
   copy_wait<0>();
 
@@ -576,79 +628,150 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   }
 }
 
-// The outputs of items that several CTAs share: CTA (c, g) adds up head g of
-// the item CTA c begins, from parts in order, so the sum never depends on who
-// came first.
+// What is left once every CTA of attend_kernel is done, by two kinds of CTAs.
+//
+// The first `joins` add up the outputs of the items that several of its `ctas`
+// CTAs share: a task is 64 dimensions of a head of one of them, its parts added
+// in a fixed order, so the sum never depends on who came first.
+//
+// The others make the entries' weights from the scores and the items' maxima
+// and sums, 32 entries a warp at a time, each entry written by the one lane it
+// falls to.  Where their entries lie they find out before attend_kernel ends:
+// neither it nor this kernel writes lengths, tables or selected pages.
 template <int D, bool F16>
-__global__ void __launch_bounds__(kThreads) join_kernel(const AttendArgs a) {
-  constexpr int COLS = D / 4, LANES = kThreads / COLS;
-  __shared__ float2 ml[kCtas];
+__global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, uint32_t ctas, uint32_t joins) {
+  constexpr int COLS = 16, LANES = kThreads / COLS, MOST = (kCtas + LANES - 1) / LANES;
+  constexpr float kShift = F16 ? 15.f : 0.f;
+  __shared__ float factor[kCtas];
   __shared__ float4 sums[kThreads];
-  pdl_wait();
-  pdl_launch_dependents();
-  const uint4 h = __ldcg(a.heads + blockIdx.x);
-  const uint32_t parts = h.y, g = blockIdx.y;
-  if (!parts) return;
-  auto part = [&](uint32_t i) { return (blockIdx.x + i) * 2 + (i == 0 ? h.z : 0u); };
-  for (uint32_t i = threadIdx.x; i < parts; i += kThreads) ml[i] = __ldcg(a.part_ml + part(i) * 8 + g);
-  __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (uint32_t i = 0; i < parts; i++) top = fmaxf(top, ml[i].x);
-  for (uint32_t i = 0; i < parts; i++) sum = fmaf(ml[i].y, fold(ml[i].x, top), sum);
-  const int col = threadIdx.x % COLS;
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (uint32_t i = threadIdx.x / COLS; i < parts; i += LANES) {
-    const float4 z = __ldcg(reinterpret_cast<const float4*>(a.part_o + ((size_t)part(i) * a.group + g) * D) + col);
-    const float f = fold(ml[i].x, top);
-    x.x = fmaf(z.x, f, x.x), x.y = fmaf(z.y, f, x.y), x.z = fmaf(z.z, f, x.z), x.w = fmaf(z.w, f, x.w);
-  }
-  sums[threadIdx.x] = x;
-  __syncthreads();
-  if (threadIdx.x >= COLS) return;
-#pragma unroll
-  for (int i = 1; i < LANES; i++) {
-    const float4 z = sums[i * COLS + col];
-    x.x += z.x, x.y += z.y, x.z += z.z, x.w += z.w;
-  }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  const uint32_t s = h.x / a.kv.kv_heads, kvh = h.x % a.kv.kv_heads;
-  *reinterpret_cast<float4*>(a.out + s * a.out_stride + (kvh * (size_t)a.group + g) * D + 4 * col) =
-      make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-  if (a.kv.weights && col == 0) a.stats[(size_t)h.x * 8 + g] = make_float2(sum == 0.f ? 0.f : top - (F16 ? 15.f : 0.f), inv);
-}
-
-// The entries' weights from the scores and the items' maxima and sums, 32
-// entries a warp at a time, each entry written by the one lane it falls to.
-__global__ void __launch_bounds__(kThreads) weigh_kernel(const AttendArgs a) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const Share sh = share_of(a, 32, kWarps);
-  if (!sh.units) return;
-  const int lane = threadIdx.x & 31;
+  __shared__ float reduce[2][kWarps];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const PagedView& v = a.kv;
-  Walk w{};
-  w.s = sh.s, w.h = sh.h;
-  load(a, w, 32);
-  w.at = -(int)sh.before;
-  for (int u = threadIdx.x >> 5; u < (int)sh.units; u += kWarps) {
-    bool more = true;
-    while (more && u >= w.at + (int)w.units) more = next(a, w, 32);
-    if (!more) return;
-    const uint32_t i = (uint32_t)(u - w.at) * 32 + lane;
-    uint32_t page, slot;
-    if (place(a, w.s, w.h, i, w.l, page, slot)) {
-      const uint64_t item = w.s * (uint64_t)v.kv_heads + w.h;
-      float sum = 0.f;
-      for (uint32_t g = 0; g < a.group; g++) {
-        const float2 st = __ldcg(a.stats + item * 8 + g);
-        sum = fmaf(exp2f(__ldcg(a.scores + (item * a.score_stride + i) * a.group + g) - st.x), st.y, sum);
+  if (blockIdx.x < joins) {
+    // The split items, in order.
+    __shared__ uint4 split[kCtas];
+    __shared__ uint32_t below[kWarps + 1];
+    pdl_wait();
+    pdl_launch_dependents();
+    uint4 h = make_uint4(0, 0, 0, 0);
+    if (t < (int)ctas) h = __ldcg(a.heads + t);
+    const uint32_t any = __ballot_sync(0xffffffffu, h.y != 0);
+    if (lane == 0) below[warp + 1] = __popc(any);
+    __syncthreads();
+    uint32_t items = 0, at = __popc(any & ((1u << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+      if (w < warp) at += below[w + 1];
+      items += below[w + 1];
+    }
+    if (h.y) split[at] = make_uint4(h.x, h.y, h.z, t);
+    __syncthreads();
+    for (uint32_t task = blockIdx.x; task < items * a.group * (D / 64); task += joins) {
+      const uint32_t chunk = task % (D / 64), g = task / (D / 64) % a.group;
+      const uint4 h = split[task / (D / 64 * a.group)];
+      const uint32_t parts = h.y, c = h.w;
+      auto part = [&](uint32_t i) { return (c + i) * 2 + (i == 0 ? h.z : 0u); };
+      const int col = t % COLS;
+      float4 x[MOST];
+#pragma unroll
+      for (int k = 0; k < MOST; k++) {
+        const uint32_t i = t / COLS + k * LANES;
+        if (i < parts)
+          x[k] = __ldcg(reinterpret_cast<const float4*>(a.part_o + ((size_t)part(i) * a.group + g) * D + chunk * 64) + col);
       }
+      const float2 ml = t < parts ? __ldcg(a.part_ml + part(t) * 8 + g) : make_float2(-INFINITY, 0.f);
+      float top = warp_max(ml.x);
+      if (lane == 0) reduce[0][warp] = top;
+      __syncthreads();
+      top = reduce[0][0];
+#pragma unroll
+      for (int w = 1; w < kWarps; w++) top = fmaxf(top, reduce[0][w]);
+      const float f = fold(ml.x, top);
+      if (t < parts) factor[t] = f;
+      float sum = warp_sum(ml.y * f);
+      if (lane == 0) reduce[1][warp] = sum;
+      __syncthreads();
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < MOST; k++) {
+        const uint32_t i = t / COLS + k * LANES;
+        if (i < parts) {
+          const float f = factor[i];
+          y.x = fmaf(x[k].x, f, y.x), y.y = fmaf(x[k].y, f, y.y), y.z = fmaf(x[k].z, f, y.z), y.w = fmaf(x[k].w, f, y.w);
+        }
+      }
+      sums[t] = y;
+      __syncthreads();
+      if (t < COLS) {
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) sum += reduce[1][w];
+#pragma unroll
+        for (int i = 1; i < LANES; i++) {
+          const float4 z = sums[i * COLS + col];
+          y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        const uint32_t s = h.x / v.kv_heads, kvh = h.x % v.kv_heads;
+        *(reinterpret_cast<float4*>(a.out + s * a.out_stride + (kvh * (size_t)a.group + g) * D + chunk * 64) + col) =
+            make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+      }
+      __syncthreads();                             // (sums, factor and reduce are used again)
+    }
+    return;
+  }
+  const Share sh = share_of(a, 32, 0, kWarps, blockIdx.x - joins, gridDim.x - joins);
+  Walk w = begin(sh, 32);
+  bool waited = false;
+  uint64_t of = ~0ull;                             // the item whose maxima and sums this lane's warp holds
+  float m = 0.f, inv = 0.f;                        // lane g: head g's
+  for (int u = warp; u < (int)sh.units; u += kWarps) {
+    bool more = true;
+    while (more && u >= w.at + (int)w.units) more = next(a, w, 32, 0);
+    const uint32_t i = (uint32_t)(u - w.at) * 32 + lane;
+    uint32_t page = 0, slot = 0;
+    const bool ok = more && place(a, w.s, w.h, i, w.l, page, slot);
+    if (!waited) {
+      pdl_wait();
+      pdl_launch_dependents();
+      waited = true;
+    }
+    const uint64_t item = w.s * (uint64_t)v.kv_heads + w.h;
+    if (more && item != of) {
+      of = item;
+      const uint4 o = __ldcg(a.origin + item);
+      if (!o.y) {
+        const float2 st = lane < (int)a.group ? __ldcg(a.stats + item * 8 + lane) : make_float2(0.f, 0.f);
+        m = st.x, inv = st.y;
+      } else {
+        // Head g's parts, a lane a part at a time.
+        for (uint32_t g = 0; g < a.group; g++) {
+          float top = -INFINITY, sum = 0.f;
+          for (uint32_t i0 = 0; i0 < o.y; i0 += 32) {
+            const uint32_t p = i0 + lane;
+            const float2 ml = p < o.y ? __ldcg(a.part_ml + ((o.x + p) * 2 + (p == 0 ? o.z : 0u)) * 8 + g)
+                                      : make_float2(-INFINITY, 0.f);
+            const float upper = fmaxf(top, warp_max(ml.x));
+            sum = fold(top, upper) * sum + warp_sum(ml.y * fold(ml.x, upper));
+            top = upper;
+          }
+          if (lane == (int)g) m = sum == 0.f ? 0.f : top - kShift, inv = sum == 0.f ? 0.f : 1.0f / sum;
+        }
+      }
+    }
+    float sum = 0.f;
+    for (uint32_t g = 0; g < a.group; g++) {
+      const float mg = __shfl_sync(0xffffffffu, m, g), ig = __shfl_sync(0xffffffffu, inv, g);
+      if (ok) sum = fmaf(exp2f(__ldcg(a.scores + (item * a.score_stride + i) * a.group + g) - mg), ig, sum);
+    }
+    if (ok) {
       float* to = v.weights + ((size_t)page * v.kv_heads + w.h) * v.page_slots + slot;
-      *to = a.decay == 0.f ? sum : fmaf(a.decay, *to, sum);
+      *to = a.decay == 0.f ? sum : fmaf(a.decay, __ldcg(to), sum);
     }
     __syncwarp();
+    if (!more) break;
   }
+  if (!waited) pdl_wait();
 }
 
 template <class T, int D>
@@ -660,20 +783,21 @@ const void* attend_of(uint32_t d, uint32_t group) {
   return d == 64 ? attend_of<T, 64>(group) : d == 128 ? attend_of<T, 128>(group) : attend_of<T, 256>(group);
 }
 template <bool F16>
-const void* join_of(uint32_t d) {
-  return d == 64    ? (const void*)join_kernel<64, F16>
-         : d == 128 ? (const void*)join_kernel<128, F16>
-                    : (const void*)join_kernel<256, F16>;
+const void* finish_of(uint32_t d) {
+  return d == 64    ? (const void*)finish_kernel<64, F16>
+         : d == 128 ? (const void*)finish_kernel<128, F16>
+                    : (const void*)finish_kernel<256, F16>;
 }
 
 // Where each part of the workspace begins; returns its whole size.
-size_t layout(const fz_paged_kv* kv, uint32_t heads, size_t (&at)[5]) {
+size_t layout(const fz_paged_kv* kv, uint32_t heads, size_t (&at)[6]) {
   const uint64_t group = heads / std::max(1u, kv->kv_heads), items = (uint64_t)kv->sequences * kv->kv_heads;
   const uint64_t entries = (uint64_t)kv->table_stride * kv->page_slots;
-  const uint64_t bytes[5] = {kCtas * 2ull * group * kv->head_dim * 4, kCtas * 2ull * 8 * 8, kCtas * 16ull,
-                             kv->weights ? items * 64 : 0, kv->weights ? items * entries * group * 4 : 0};
+  const uint64_t bytes[6] = {kCtas * 2ull * group * kv->head_dim * 4, kCtas * 2ull * 8 * 8, kCtas * 16ull,
+                             kv->weights ? items * 16 : 0, kv->weights ? items * 64 : 0,
+                             kv->weights ? items * entries * group * 4 : 0};
   size_t end = 0;
-  for (int i = 0; i < 5; i++) {
+  for (int i = 0; i < 6; i++) {
     at[i] = end;
     end += (bytes[i] + 255) / 256 * 256;
   }
@@ -684,7 +808,7 @@ size_t layout(const fz_paged_kv* kv, uint32_t heads, size_t (&at)[5]) {
 }  // namespace fz
 
 extern "C" size_t fz_paged_attention_workspace(const fz_paged_kv* kv, uint32_t heads) {
-  size_t at[5];
+  size_t at[6];
   return kv ? fz::layout(kv, heads, at) : 0;
 }
 
@@ -722,14 +846,15 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   a.blocks = query->blocks, a.group = heads / kv->kv_heads, a.top = query->top, a.window = query->window;
   a.scale_log2e = (float)((double)query->scale * 1.4426950408889634);
   a.decay = query->decay;
-  size_t at[5];
+  size_t at[6];
   layout(kv, heads, at);
   char* w = static_cast<char*>(query->workspace);
   a.part_o = reinterpret_cast<float*>(w + at[0]);
   a.part_ml = reinterpret_cast<float2*>(w + at[1]);
   a.heads = reinterpret_cast<uint4*>(w + at[2]);
-  a.stats = reinterpret_cast<float2*>(w + at[3]);
-  a.scores = reinterpret_cast<float*>(w + at[4]);
+  a.origin = reinterpret_cast<uint4*>(w + at[3]);
+  a.stats = reinterpret_cast<float2*>(w + at[4]);
+  a.scores = reinterpret_cast<float*>(w + at[5]);
   a.score_stride = (uint64_t)kv->table_stride * kv->page_slots;
   // The longest list an item can have, in tiles: with at most one a warp,
   // items stay whole (no join, and no CTA needs every length).
@@ -747,13 +872,9 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   if ((st = paged_launch(f16 ? attend_of<F16>(d, a.group) : attend_of<Bf16>(d, a.group), dim3(grid), dim3(kThreads), kSmem, 1,
                          args, stream)))
     return st;
-  if (!a.whole &&
-      (st = paged_launch(f16 ? join_of<true>(d) : join_of<false>(d), dim3(grid, a.group), dim3(kThreads), 0, 1, args, stream)))
-    return st;
-  if (a.kv.weights) {
-    const uint64_t units = items * ((most + 31) / 32);
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>(4 * kCtas, (units + kWarps - 1) / kWarps);
-    st = paged_launch((const void*)weigh_kernel, dim3(blocks), dim3(kThreads), 0, 1, args, stream);
-  }
-  return st;
+  uint32_t joins = a.whole ? 0u : std::min(2 * kCtas, grid * a.group * (d / 64)), weighs = 0, ctas = grid;
+  if (a.kv.weights) weighs = (uint32_t)std::min<uint64_t>(4 * kCtas, (items * ((most + 31) / 32) + kWarps - 1) / kWarps);
+  if (!joins && !weighs) return FZ_OK;
+  void* left[] = {&a, &ctas, &joins};
+  return paged_launch(f16 ? finish_of<true>(d) : finish_of<false>(d), dim3(joins + weighs), dim3(kThreads), 0, 1, left, stream);
 }
