@@ -30,7 +30,7 @@ struct AttendArgs {
   uint4* heads;            // [kCtas] the split item a CTA begins: {item, CTAs, its slot, 0}
   uint4* origin;           // [items] where an item's outputs are, for the weights: {first CTA, CTAs, its slot, 0}
   float2* stats;           // [items][8] an unsplit item's maximum and reciprocal sum, for the weights
-  float* scores;           // [items][score_stride][group] in log2 units, for the weights
+  float* scores;           // [items][group][score_stride] in log2 units, for the weights
   uint64_t score_stride;
 };
 
@@ -74,63 +74,93 @@ FZ_DEV bool place(const AttendArgs& a, uint32_t s, uint32_t h, uint32_t i, const
   return false;
 }
 
-// CTA `cta` of `ctas`' share of all items' units (`unit` entries a unit, and
-// before each item `extra` that stand for what beginning an item costs), in
-// order of sequence and KV head: a contiguous run of ceil(all / ctas) units, at
-// least `least`, so that every CTA takes as long as the others whatever the
-// lengths.  Called by the whole block.
+constexpr uint32_t kBegin = kWarps;    // units that beginning an item costs
+constexpr uint32_t kJoin = kWarps;     // units that adding up shared items costs
+
+// A CTA's share of all items' units (`unit` entries a unit), in order of
+// sequence and KV head: a contiguous run of ceil(all / CTAs) units, so that
+// every CTA reads as much as the others whatever the lengths.  Where a CTA has
+// several tiles a warp, `extra` units before each item stand for what beginning
+// it costs (measured at 8 x 32,768 entries of one KV head: CTAs with two items
+// ended 12 us after the others; counted as 8 units, 55 -> 40 us).  Where whole
+// items, the same number a CTA, take no longer than that and the joining (many
+// items of like length), items are not cut.  Called by the whole block.
 struct Share {
-  uint32_t units;          // this CTA's
-  uint32_t s, h;           // the item of its first unit
+  uint32_t units, items;   // this CTA's; the one that does not count is large
+  uint32_t extra;
+  uint32_t s, h;           // the first item
   int at;                  // where that item's entries begin, from the CTA's first unit
   List l;                  // its list
   uint64_t first, per;
 };
-FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit, uint32_t extra, uint32_t least, uint32_t cta, uint32_t ctas) {
-  __shared__ uint64_t sum[kWarps];
+FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit) {
+  __shared__ uint64_t sums[kWarps];
+  __shared__ uint2 counts[kWarps];
   __shared__ Share found;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const uint32_t S = a.kv.sequences, run = (S + kThreads - 1) / kThreads, s0 = min(S, t * run), s1 = min(S, s0 + run);
-  uint64_t mine = 0;
+  const uint32_t ctas = gridDim.x, KV = a.kv.kv_heads;
+  uint64_t tiles = 0;
+  uint32_t some = 0, most = 0;
   List l{};
   for (uint32_t s = s0; s < s1; s++) {
     l = list_of(a, s);
-    if (l.count) mine += (l.count + unit - 1) / unit + extra;
+    const uint32_t u = (l.count + unit - 1) / unit;
+    tiles += u;
+    some += u != 0;
+    most = max(most, u);
   }
-  uint64_t upto = mine;
+  uint64_t upto = tiles;
+  uint32_t some_upto = some;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
+    const uint32_t y = __shfl_up_sync(0xffffffffu, some_upto, o);
+    if (lane >= o) upto += x, some_upto += y;
   }
-  if (lane == 31) sum[warp] = upto;
-  if (t == 0) found.units = 0;
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 31) sums[warp] = upto, counts[warp] = make_uint2(some_upto, most);
+  if (t == 0) found.units = found.items = 0;
   __syncthreads();
   uint64_t all = 0, before = 0;
+  uint32_t any = 0, some_before = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; w++) {
-    if (w < warp) before += sum[w];
-    all += sum[w];
+    if (w < warp) before += sums[w], some_before += counts[w].x;
+    all += sums[w];
+    any += counts[w].x;
+    most = max(most, counts[w].y);
   }
-  const uint64_t KV = a.kv.kv_heads;
-  all *= KV;
-  before = (before + upto - mine) * KV;
+  before += upto - tiles;
+  some_before += some_upto - some;
+  const uint64_t items = (uint64_t)any * KV;
+  const uint32_t extra = all * KV >= 2ull * kWarps * ctas ? kBegin : 0u;
+  all = all * KV + items * extra;
   const uint64_t even = (all >> 32) ? (all + ctas - 1) / ctas : ((uint32_t)all + (ctas - 1)) / ctas;
-  const uint64_t per = max((uint64_t)least, even), first = cta * per;
-  if (first < all && before <= first && first < before + mine * KV) {
+  const uint64_t per = max((uint64_t)kWarps, even);
+  const uint64_t each = (items >> 32) ? (items + ctas - 1) / ctas : ((uint32_t)items + (ctas - 1)) / ctas;
+  const bool whole = each * (most + extra) <= per + kJoin;
+  // This thread's sequences, in units or in items.
+  const uint64_t from = whole ? (uint64_t)some_before * KV : (before + (uint64_t)some_before * extra) * KV;
+  const uint64_t length = whole ? (uint64_t)some * KV : (tiles + (uint64_t)some * extra) * KV;
+  const uint64_t first = blockIdx.x * (whole ? each : per);
+  if (length && from <= first && first < from + length) {
+    uint64_t base = from;
     uint32_t s = s0, u;
     for (;; s++) {
       if (run > 1) l = list_of(a, s);
-      u = l.count ? (l.count + unit - 1) / unit + extra : 0u;
-      if (first < before + u * KV) break;
-      before += u * KV;
+      u = l.count ? (whole ? 1u : (l.count + unit - 1) / unit + extra) : 0u;
+      if (first < base + (uint64_t)u * KV) break;
+      base += (uint64_t)u * KV;
     }
-    const uint64_t in = first - before;
+    const uint64_t in = first - base;
     found.h = KV == 1 ? 0u : (uint32_t)(in / u);
-    found.at = (int)(extra + (int64_t)found.h * u - (int64_t)in);
+    found.at = whole ? 0 : (int)(extra + (int64_t)found.h * u - (int64_t)in);
+    found.extra = extra;
     found.l = l;
     found.s = s;
-    found.units = (uint32_t)min(per, all - first);
+    found.items = whole ? (uint32_t)min(each, items - first) : 0xFFFFFFFFu;
+    found.units = whole ? 0x7FFFFFFFu : (uint32_t)min(per, all - first);
     found.first = first;
     found.per = per;
   }
@@ -143,6 +173,7 @@ FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit, uint32_t extra, uint32
 struct Walk {
   uint32_t s, h, units;
   int at;
+  uint32_t index;          // items before it in the CTA
   List l;
 };
 FZ_DEV void load(const AttendArgs& a, Walk& w, uint32_t unit) {
@@ -154,6 +185,7 @@ FZ_DEV void load(const AttendArgs& a, Walk& w, uint32_t unit) {
 // empty ones).
 FZ_DEV bool next(const AttendArgs& a, Walk& w, uint32_t unit, uint32_t extra) {
   w.at += (int)(w.units + extra);
+  w.index++;
   if (++w.h < a.kv.kv_heads && w.units) return true;
   w.h = 0;
   w.units = 0;
@@ -172,7 +204,7 @@ FZ_DEV bool next(const AttendArgs& a, Walk& w, uint32_t unit, uint32_t extra) {
 
 // The item a share begins with.
 FZ_DEV Walk begin(const Share& sh, uint32_t unit) {
-  return Walk{sh.s, sh.h, (sh.l.count + unit - 1) / unit, sh.at, sh.l};
+  return Walk{sh.s, sh.h, (sh.l.count + unit - 1) / unit, sh.at, 0, sh.l};
 }
 
 FZ_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -282,33 +314,31 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   pdl_wait();
   pdl_launch_dependents();
 
-  // This CTA's items: a share of the units, or whole items.
+  // This CTA's items: a share of all units, or where no item has more than one
+  // tile a warp, whole items by their number alone.
   Walk seg{};
-  uint32_t units = 0xFFFFFFFFu, last_item = 0;     // units, or the item after the last
+  uint32_t units = 0x7FFFFFFFu, items = 0xFFFFFFFFu, last_item = 0xFFFFFFFFu, extra = 0;
   uint64_t first = 0, per = 1;
   bool some;
   if (a.whole) {
-    const uint64_t items = (uint64_t)v.sequences * KV;
-    const uint32_t i0 = (uint32_t)(items * blockIdx.x / gridDim.x);
-    last_item = (uint32_t)(items * (blockIdx.x + 1) / gridDim.x);
+    const uint64_t all = (uint64_t)v.sequences * KV;
+    const uint32_t i0 = (uint32_t)(all * blockIdx.x / gridDim.x);
+    last_item = (uint32_t)(all * (blockIdx.x + 1) / gridDim.x);
     seg.s = i0 / KV, seg.h = i0 % KV;
     some = i0 < last_item;
     if (some) {
       load(a, seg, KT);
-      if (!seg.units) {
-        some = next(a, seg, KT, kWarps);
-        seg.at = 0;
-      }
+      if (!seg.units) some = next(a, seg, KT, 0);
     }
   } else {
-    const Share sh = share_of(a, KT, kWarps, 2 * kWarps, blockIdx.x, gridDim.x);
-    units = sh.units;
+    const Share sh = share_of(a, KT);
+    units = sh.units, items = sh.items, extra = sh.extra;
     some = units != 0;
     first = sh.first, per = sh.per;
     if (some) seg = begin(sh, KT);
     if (threadIdx.x == 0) a.heads[blockIdx.x] = make_uint4(0, 0, 0, 0);
   }
-  auto mine = [&](const Walk& w) { return a.whole ? w.s * KV + w.h < last_item : w.at < (int)units; };
+  auto mine = [&](const Walk& w) { return w.at < (int)units && w.index < items && w.s * KV + w.h < last_item; };
 
   // An item's q, a few floats a thread, asked for an item ahead: a load waits
   // behind all the copies in flight, some 3 us.
@@ -376,9 +406,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
     while (w.any) {
       // (The units before an item's first hold nothing.)
       if (unit_ahead < ahead.at) unit_ahead += (ahead.at - unit_ahead + kWarps - 1) / kWarps * kWarps;
-      w.any = mine(ahead) && (a.whole || unit_ahead < (int)units);
+      w.any = mine(ahead) && unit_ahead < (int)units;
       if (!w.any || unit_ahead < ahead.at + (int)ahead.units) break;
-      w.any = more = next(a, ahead, KT, kWarps);
+      w.any = more = next(a, ahead, KT, extra);
     }
     w.valid = 0;
 #pragma unroll
@@ -416,11 +446,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   int unit = warp;
 
   while (some && mine(seg)) {
-    const int from = max(seg.at, 0), to = min(seg.at + (int)seg.units, (int)min(units, 0x7FFFFFFFu));
+    const int from = max(seg.at, 0), to = min(seg.at + (int)seg.units, (int)units);
     if (unit < seg.at) unit += (seg.at - unit + kWarps - 1) / kWarps * kWarps;
     put_q();
     Walk after = seg;
-    const bool then = next(a, after, KT, kWarps);
+    const bool then = next(a, after, KT, extra);
     if (then && mine(after)) ask_q(after);
     const float c0 = qc[(2 * t4) % GP], c1 = qc[(2 * t4 + 1) % GP];
     float o[KS][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
@@ -481,13 +511,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
         t1 = fmaxf(t1, fmaxf(s[ms][1], s[ms][3]));
       }
       if (v.weights && 2 * t4 < GP) {
-        const uint64_t e = (seg.s * (uint64_t)KV + seg.h) * a.score_stride + (uint32_t)(unit - seg.at) * KT;
+        float* to = a.scores + ((seg.s * (uint64_t)KV + seg.h) * G + 2 * t4) * a.score_stride + (uint32_t)(unit - seg.at) * KT + g4;
 #pragma unroll
         for (int x = 0; x < 2 * MS; x++)
 #pragma unroll
           for (int c = 0; c < 2; c++)
             if ((valid >> (8 * x + g4)) & 1 && 2 * t4 + c < G)
-              a.scores[(e + 8 * x + g4) * G + 2 * t4 + c] = s[x / 2][2 * (x & 1) + c];
+              to[c * a.score_stride + 8 * x] = s[x / 2][2 * (x & 1) + c];
       }
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) {
@@ -635,11 +665,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
 // in a fixed order, so the sum never depends on who came first.
 //
 // The others make the entries' weights from the scores and the items' maxima
-// and sums, 32 entries a warp at a time, each entry written by the one lane it
-// falls to.  Where their entries lie they find out before attend_kernel ends:
-// neither it nor this kernel writes lengths, tables or selected pages.
+// and sums, 128 entries a warp at a time, four a lane, each entry written by the
+// one lane it falls to.  Where their entries lie they find out before
+// attend_kernel ends: neither it nor this kernel writes lengths, tables or
+// selected pages.
+constexpr int kWeighed = 128;
 template <int D, bool F16>
-__global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, uint32_t ctas, uint32_t joins) {
+__global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, uint32_t ctas, uint32_t joins, uint32_t pieces) {
   constexpr int COLS = 16, LANES = kThreads / COLS, MOST = (kCtas + LANES - 1) / LANES;
   constexpr float kShift = F16 ? 15.f : 0.f;
   __shared__ float factor[kCtas];
@@ -720,56 +752,80 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, ui
     }
     return;
   }
-  const Share sh = share_of(a, 32, 0, kWarps, blockIdx.x - joins, gridDim.x - joins);
-  Walk w = begin(sh, 32);
   bool waited = false;
-  uint64_t of = ~0ull;                             // the item whose maxima and sums this lane's warp holds
-  float m = 0.f, inv = 0.f;                        // lane g: head g's
-  for (int u = warp; u < (int)sh.units; u += kWarps) {
-    bool more = true;
-    while (more && u >= w.at + (int)w.units) more = next(a, w, 32, 0);
-    const uint32_t i = (uint32_t)(u - w.at) * 32 + lane;
-    uint32_t page = 0, slot = 0;
-    const bool ok = more && place(a, w.s, w.h, i, w.l, page, slot);
+  uint64_t of = ~0ull;                             // the item whose maxima and sums this warp holds
+  float m = 0.f, inv = 0.f;                        // lanes 4 g ..: head g's
+  const uint64_t units = (uint64_t)v.sequences * v.kv_heads * pieces;
+  for (uint64_t u = (blockIdx.x - joins) * kWarps + warp; u < units; u += (uint64_t)(gridDim.x - joins) * kWarps) {
+    const uint64_t item = u / pieces;
+    const uint32_t s = (uint32_t)(item / v.kv_heads), kvh = (uint32_t)(item % v.kv_heads);
+    const List l = list_of(a, s);
+    const uint32_t i0 = (uint32_t)(u - item * pieces) * kWeighed;
+    if (i0 >= l.count) continue;
+    const uint32_t i = i0 + 4 * lane;
+    float* to[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      uint32_t page, slot;
+      const bool ok = place(a, s, kvh, i + c, l, page, slot);
+      to[c] = ok ? v.weights + ((size_t)page * v.kv_heads + kvh) * v.page_slots + slot : nullptr;
+    }
     if (!waited) {
       pdl_wait();
       pdl_launch_dependents();
       waited = true;
     }
-    const uint64_t item = w.s * (uint64_t)v.kv_heads + w.h;
-    if (more && item != of) {
+    float4 x[8];
+    float old[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < 8; g++)
+      if (g < (int)a.group && i < l.count)
+        x[g] = __ldcg(reinterpret_cast<const float4*>(a.scores + (item * a.group + g) * a.score_stride + i));
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+      if (a.decay != 0.f && to[c]) old[c] = __ldcg(to[c]);
+    if (item != of) {
       of = item;
+      // Lanes 4 g .. 4 g + 3: every fourth of head g's parts (an unsplit item has its maximum and reciprocal sum).
       const uint4 o = __ldcg(a.origin + item);
+      const uint32_t g = lane / 4;
       if (!o.y) {
-        const float2 st = lane < (int)a.group ? __ldcg(a.stats + item * 8 + lane) : make_float2(0.f, 0.f);
+        const float2 st = g < a.group ? __ldcg(a.stats + item * 8 + g) : make_float2(0.f, 0.f);
         m = st.x, inv = st.y;
       } else {
-        // Head g's parts, a lane a part at a time.
-        for (uint32_t g = 0; g < a.group; g++) {
-          float top = -INFINITY, sum = 0.f;
-          for (uint32_t i0 = 0; i0 < o.y; i0 += 32) {
-            const uint32_t p = i0 + lane;
-            const float2 ml = p < o.y ? __ldcg(a.part_ml + ((o.x + p) * 2 + (p == 0 ? o.z : 0u)) * 8 + g)
-                                      : make_float2(-INFINITY, 0.f);
-            const float upper = fmaxf(top, warp_max(ml.x));
-            sum = fold(top, upper) * sum + warp_sum(ml.y * fold(ml.x, upper));
-            top = upper;
-          }
-          if (lane == (int)g) m = sum == 0.f ? 0.f : top - kShift, inv = sum == 0.f ? 0.f : 1.0f / sum;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+        for (uint32_t p = lane & 3; p < o.y; p += 4) {
+          const float2 ml = g < a.group ? __ldcg(a.part_ml + ((o.x + p) * 2 + (p == 0 ? o.z : 0u)) * 8 + g)
+                                        : make_float2(-INFINITY, 0.f);
+          const float upper = fmaxf(top, ml.x);
+          sum = fold(top, upper) * sum + ml.y * fold(ml.x, upper);
+          top = upper;
         }
+        __syncwarp();
+        float upper = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        upper = fmaxf(upper, __shfl_xor_sync(0xffffffffu, upper, 2));
+        sum *= fold(top, upper);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        m = sum == 0.f ? 0.f : upper - kShift, inv = sum == 0.f ? 0.f : 1.0f / sum;
       }
     }
-    float sum = 0.f;
-    for (uint32_t g = 0; g < a.group; g++) {
-      const float mg = __shfl_sync(0xffffffffu, m, g), ig = __shfl_sync(0xffffffffu, inv, g);
-      if (ok) sum = fmaf(exp2f(__ldcg(a.scores + (item * a.score_stride + i) * a.group + g) - mg), ig, sum);
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < 8; g++) {
+      const float mg = __shfl_sync(0xffffffffu, m, 4 * g), ig = __shfl_sync(0xffffffffu, inv, 4 * g);
+      if (g < (int)a.group) {
+        sum[0] = fmaf(exp2f(x[g].x - mg), ig, sum[0]);
+        sum[1] = fmaf(exp2f(x[g].y - mg), ig, sum[1]);
+        sum[2] = fmaf(exp2f(x[g].z - mg), ig, sum[2]);
+        sum[3] = fmaf(exp2f(x[g].w - mg), ig, sum[3]);
+      }
     }
-    if (ok) {
-      float* to = v.weights + ((size_t)page * v.kv_heads + w.h) * v.page_slots + slot;
-      *to = a.decay == 0.f ? sum : fmaf(a.decay, __ldcg(to), sum);
-    }
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+      if (to[c]) *to[c] = fmaf(a.decay, old[c], sum[c]);
     __syncwarp();
-    if (!more) break;
   }
   if (!waited) pdl_wait();
 }
@@ -792,7 +848,7 @@ const void* finish_of(uint32_t d) {
 // Where each part of the workspace begins; returns its whole size.
 size_t layout(const fz_paged_kv* kv, uint32_t heads, size_t (&at)[6]) {
   const uint64_t group = heads / std::max(1u, kv->kv_heads), items = (uint64_t)kv->sequences * kv->kv_heads;
-  const uint64_t entries = (uint64_t)kv->table_stride * kv->page_slots;
+  const uint64_t entries = ((uint64_t)kv->table_stride * kv->page_slots + kWeighed - 1) / kWeighed * kWeighed;
   const uint64_t bytes[6] = {kCtas * 2ull * group * kv->head_dim * 4, kCtas * 2ull * 8 * 8, kCtas * 16ull,
                              kv->weights ? items * 16 : 0, kv->weights ? items * 64 : 0,
                              kv->weights ? items * entries * group * 4 : 0};
@@ -855,10 +911,11 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   a.origin = reinterpret_cast<uint4*>(w + at[3]);
   a.stats = reinterpret_cast<float2*>(w + at[4]);
   a.scores = reinterpret_cast<float*>(w + at[5]);
-  a.score_stride = (uint64_t)kv->table_stride * kv->page_slots;
+  const uint64_t entries = (uint64_t)kv->table_stride * kv->page_slots;
+  a.score_stride = (entries + kWeighed - 1) / kWeighed * kWeighed;
   // The longest list an item can have, in tiles: with at most one a warp,
   // items stay whole (no join, and no CTA needs every length).
-  uint64_t most = a.score_stride;
+  uint64_t most = entries;
   if (a.blocks) most = std::min<uint64_t>(most, (uint64_t)a.top * kv->page_slots);
   else if (a.window) most = std::min<uint64_t>(most, a.window);
   const uint32_t tile = 4096 / kv->head_dim;
@@ -872,9 +929,10 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   if ((st = paged_launch(f16 ? attend_of<F16>(d, a.group) : attend_of<Bf16>(d, a.group), dim3(grid), dim3(kThreads), kSmem, 1,
                          args, stream)))
     return st;
-  uint32_t joins = a.whole ? 0u : std::min(2 * kCtas, grid * a.group * (d / 64)), weighs = 0, ctas = grid;
-  if (a.kv.weights) weighs = (uint32_t)std::min<uint64_t>(4 * kCtas, (items * ((most + 31) / 32) + kWarps - 1) / kWarps);
+  uint32_t joins = a.whole ? 0u : std::min(4 * kCtas, grid * a.group * (d / 64)), weighs = 0, ctas = grid;
+  uint32_t pieces = (uint32_t)((most + kWeighed - 1) / kWeighed);
+  if (a.kv.weights) weighs = (uint32_t)std::min<uint64_t>(8 * kCtas, (items * pieces + kWarps - 1) / kWarps);
   if (!joins && !weighs) return FZ_OK;
-  void* left[] = {&a, &ctas, &joins};
+  void* left[] = {&a, &ctas, &joins, &pieces};
   return paged_launch(f16 ? finish_of<true>(d) : finish_of<false>(d), dim3(joins + weighs), dim3(kThreads), 0, 1, left, stream);
 }
