@@ -2,6 +2,7 @@
 // one pass) and the pages' key bounds.
 #include "paged.cuh"
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -104,79 +105,102 @@ struct AppendArgs {
   fz_paged_rows r;
 };
 
-// One warp a (row, head): D / 64 ... a lane holds D / 64 pairs (i, i + D / 2).
-// The sum of squares and the norm in f32, the angle's turns in f64 (position
-// x turns loses its fraction in f32 past a few thousand positions), its
-// fraction's sine and cosine in f32.
-template <class T, int D>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
-  constexpr int P = D / 64;                    // pairs a lane
+// Norm, rotation and store in one pass over a row's heads: memory bound, 4 bytes
+// read a value and 2 or 4 written.  A head is D / 8 lanes, four values of each
+// half a lane (the rotation's pairs in one lane, 16-byte accesses); a warp takes
+// PASSES times 256 / D heads of one row, all their loads first, so the row's
+// sines and cosines are made once for them.  The sum of squares and the norm in
+// f32; the angle's turns in f64 (position x turns loses its fraction in f32 past
+// a few thousand positions), its fraction's sine and cosine in f32.  4,095 rows
+// of 8 + 2 + 2 heads of 256: 92 MB.
+template <class T, int D, int PASSES>
+__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a, uint32_t warps_a_row) {
+  constexpr int LANES = D / 8, HEADS = 32 / LANES;
   pdl_wait();
+  pdl_launch_dependents();
   const fz_paged_rows& r = a.r;
   const PagedView& v = a.kv;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, part = lane % LANES;
   const uint32_t heads = r.heads + 2 * v.kv_heads;
-  const uint64_t item = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const uint64_t row = item / heads;
+  const uint64_t warp = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint64_t row = (warp >> 32) ? warp / warps_a_row : (uint32_t)warp / warps_a_row;
   if (row >= r.rows) return;
-  const uint32_t head = (uint32_t)(item % heads);
-  const uint32_t seq = r.sequence ? r.sequence[row] : (uint32_t)row;
-  if (seq == FZ_PAGED_NONE) return;
-  const uint32_t index = r.index[row];
-  const bool query = head < r.heads, value = head >= r.heads + v.kv_heads;
-  const uint32_t h = query ? head : value ? head - r.heads - v.kv_heads : head - r.heads;
-  const float* src = (query ? r.q + row * r.q_stride : value ? r.v + row * r.v_stride : r.k + row * r.k_stride) + (size_t)h * D;
-  float x[P], y[P];
+  const uint32_t head0 = (uint32_t)(warp - row * warps_a_row) * (PASSES * HEADS) + lane / LANES;
+  float4 x[PASSES], y[PASSES];
 #pragma unroll
-  for (int i = 0; i < P; i++) x[i] = src[lane * P + i], y[i] = src[D / 2 + lane * P + i];
-  if (!value) {
-    const float* gain = query ? r.q_gain : r.k_gain;
-    if (gain) {
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < P; i++) s = fmaf(x[i], x[i], fmaf(y[i], y[i], s));
-      s = warp_sum(s);
-      const float inv = rsqrtf(fmaf(s, 1.0f / D, r.eps));
-#pragma unroll
-      for (int i = 0; i < P; i++) x[i] = x[i] * inv * gain[lane * P + i], y[i] = y[i] * inv * gain[D / 2 + lane * P + i];
+  for (int p = 0; p < PASSES; p++) {
+    const uint32_t head = head0 + p * HEADS;
+    if (head < heads) {
+      const bool query = head < r.heads, value = head >= r.heads + v.kv_heads;
+      const float* src = query   ? r.q + row * r.q_stride + (size_t)head * D
+                         : value ? r.v + row * r.v_stride + (size_t)(head - r.heads - v.kv_heads) * D
+                                 : r.k + row * r.k_stride + (size_t)(head - r.heads) * D;
+      x[p] = __ldcs(reinterpret_cast<const float4*>(src) + part);
+      y[p] = __ldcs(reinterpret_cast<const float4*>(src + D / 2) + part);
+    } else {
+      x[p] = y[p] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    if (r.turns) {
-      const double pos = (double)(r.position ? r.position[row] : index);
+  }
+  const uint32_t seq = r.sequence ? r.sequence[row] : (uint32_t)row;
+  const uint32_t index = r.index[row];
+  if (seq == FZ_PAGED_NONE) return;
+  const bool in_table = seq < v.sequences && index < v.table_stride * v.page_slots;
+  const uint32_t page = in_table ? v.table[(size_t)seq * v.table_stride + index / v.page_slots] : 0u;
+  const uint32_t slot = index % v.page_slots;
+  float sn[4], cs[4];
+  if (r.turns) {
+    const double pos = (double)(r.position ? r.position[row] : index);
+    const double2 t0 = reinterpret_cast<const double2*>(r.turns)[2 * part], t1 = reinterpret_cast<const double2*>(r.turns)[2 * part + 1];
+    const double turns[4] = {pos * t0.x, pos * t0.y, pos * t1.x, pos * t1.y};
 #pragma unroll
-      for (int i = 0; i < P; i++) {
-        const double t = pos * r.turns[lane * P + i];
-        float sn, cs;
-        sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
-        const float u = x[i], w = y[i];
-        x[i] = u * cs - w * sn;
-        y[i] = u * sn + w * cs;
+    for (int i = 0; i < 4; i++) sincospif(2.0f * (float)(turns[i] - rint(turns[i])), &sn[i], &cs[i]);
+  }
+#pragma unroll
+  for (int p = 0; p < PASSES; p++) {
+    const uint32_t head = head0 + p * HEADS;
+    const bool query = head < r.heads, value = head >= r.heads + v.kv_heads, any = head < heads;
+    const float* gain = query ? r.q_gain : r.k_gain;
+    const bool normed = any && !value && gain;
+    float xs[4] = {x[p].x, x[p].y, x[p].z, x[p].w}, ys[4] = {y[p].x, y[p].y, y[p].z, y[p].w};
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum = fmaf(xs[i], xs[i], fmaf(ys[i], ys[i], sum));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (!any) continue;
+    if (normed) {
+      const float inv = rsqrtf(fmaf(sum, 1.0f / D, r.eps));
+      const float4 gx = reinterpret_cast<const float4*>(gain)[part], gy = reinterpret_cast<const float4*>(gain + D / 2)[part];
+      const float g0[4] = {gx.x, gx.y, gx.z, gx.w}, g1[4] = {gy.x, gy.y, gy.z, gy.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) xs[i] = xs[i] * inv * g0[i], ys[i] = ys[i] * inv * g1[i];
+    }
+    if (!value && r.turns) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float u = xs[i], w = ys[i];
+        xs[i] = u * cs[i] - w * sn[i];
+        ys[i] = u * sn[i] + w * cs[i];
       }
     }
-  }
-  if (query) {
-    float* out = r.q_out + row * r.q_out_stride + (size_t)h * D;
-#pragma unroll
-    for (int i = 0; i < P; i++) out[lane * P + i] = x[i], out[D / 2 + lane * P + i] = y[i];
-    return;
-  }
-  if (seq >= v.sequences || index >= v.table_stride * v.page_slots) {
-    if (lane == 0) note(v, FZ_PAGED_BAD_ROW);
-    return;
-  }
-  const uint32_t page = v.table[(size_t)seq * v.table_stride + index / v.page_slots], slot = index % v.page_slots;
-  if (page >= v.pages) {
-    if (lane == 0) note(v, FZ_PAGED_BAD_PAGE);
-    return;
-  }
-  uint16_t* dst = (value ? v.values : v.keys) + element(v, page, slot, h);
-#pragma unroll
-  for (int i = 0; i < P; i++) {
-    dst[lane * P + i] = (uint16_t)T::pack(x[i], 0.f);
-    dst[D / 2 + lane * P + i] = (uint16_t)T::pack(y[i], 0.f);
-  }
-  if (lane == 0) {
-    if (!value && v.weights) v.weights[((size_t)page * v.kv_heads + h) * v.page_slots + slot] = 0.f;
-    if (!value && h == 0) atomicMax(v.lengths + seq, index + 1);
+    if (query) {
+      float* out = r.q_out + row * r.q_out_stride + (size_t)head * D;
+      reinterpret_cast<float4*>(out)[part] = make_float4(xs[0], xs[1], xs[2], xs[3]);
+      reinterpret_cast<float4*>(out + D / 2)[part] = make_float4(ys[0], ys[1], ys[2], ys[3]);
+      continue;
+    }
+    const uint32_t h = value ? head - r.heads - v.kv_heads : head - r.heads;
+    if (!in_table || page >= v.pages) {
+      if (part == 0) note(v, in_table ? FZ_PAGED_BAD_PAGE : FZ_PAGED_BAD_ROW);
+      continue;
+    }
+    uint16_t* dst = (value ? v.values : v.keys) + element(v, page, slot, h);
+    reinterpret_cast<uint2*>(dst)[part] = make_uint2(T::pack(xs[0], xs[1]), T::pack(xs[2], xs[3]));
+    reinterpret_cast<uint2*>(dst + D / 2)[part] = make_uint2(T::pack(ys[0], ys[1]), T::pack(ys[2], ys[3]));
+    if (part == 0 && !value) {
+      if (v.weights) v.weights[((size_t)page * v.kv_heads + h) * v.page_slots + slot] = 0.f;
+      if (h == 0) atomicMax(v.lengths + seq, index + 1);
+    }
   }
 }
 
@@ -212,40 +236,85 @@ FZ_DEV uint32_t most2<Bf16>(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// One warp a (sequence, logical page, KV head), a lane D / 64 pairs of dimensions.
+// A page and KV head is D / 8 lanes, 16 bytes of each key a lane, the other
+// lanes of a warp (256 / D of them) every other slot; AHEAD slots' loads in
+// flight a lane.  A warp takes pages of the run first .. length - 1 of all
+// sequences in order, so the work is even whatever the lengths: the pages of
+// each 32 sequences are counted by one look at their lengths.  Memory bound:
+// every key is read once, 2 / page_slots of that written.
 template <class T, int D>
 __global__ void __launch_bounds__(256) bounds_kernel(const BoundsArgs a) {
-  constexpr int P = D / 64;
+  constexpr int LANES = D / 8, ROWS = 32 / LANES, AHEAD = 8;
   pdl_wait();
+  pdl_launch_dependents();
   const PagedView& v = a.kv;
-  const int lane = threadIdx.x & 31;
-  const uint64_t items = (uint64_t)v.table_stride * v.kv_heads;
-  const uint64_t item = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= items) return;
-  const uint32_t logical = (uint32_t)(item / v.kv_heads), h = (uint32_t)(item % v.kv_heads);
-  for (uint32_t s = blockIdx.y; s < v.sequences; s += gridDim.y) {
-    const uint32_t n = held(v, s), j0 = logical * v.page_slots;
-    if (lane == 0 && item == 0 && v.lengths[s] > n) note(v, FZ_PAGED_BAD_LENGTH);
-    if (j0 >= n || (a.first && a.first[s] >= n) || (a.first && a.first[s] >= j0 + v.page_slots)) continue;
-    const uint32_t page = v.table[(size_t)s * v.table_stride + logical];
-    if (page >= v.pages) {
-      if (lane == 0) note(v, FZ_PAGED_BAD_PAGE);
-      continue;
+  const int lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES;
+  const uint64_t stride = (uint64_t)gridDim.x * 8;
+  uint64_t item = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);       // page and head, counted over all sequences
+  uint64_t before = 0;                                                 // of sequences s0 ..
+  for (uint32_t s0 = 0; s0 < v.sequences; s0 += 32) {
+    // Lane s: sequence s0 + s's entries, first touched page and number of pages times heads.
+    const uint32_t s = s0 + lane;
+    uint32_t n = 0, page0 = 0;
+    uint64_t count = 0;
+    if (s < v.sequences) {
+      n = held(v, s);
+      if (v.lengths[s] > n) note(v, FZ_PAGED_BAD_LENGTH);
+      const uint32_t first = a.first ? a.first[s] : 0u;
+      page0 = first / v.page_slots;
+      if (first < n) count = (uint64_t)((n + v.page_slots - 1) / v.page_slots - page0) * v.kv_heads;
     }
-    uint32_t lo[P], hi[P];
-    const uint32_t slots = min(v.page_slots, n - j0);
-    for (uint32_t i = 0; i < slots; i++) {
-      const uint32_t* k = reinterpret_cast<const uint32_t*>(v.keys + element(v, page, i, h));
+    uint64_t upto = count;
 #pragma unroll
-      for (int c = 0; c < P; c++) {
-        const uint32_t w = k[lane + 32 * c];
-        lo[c] = i ? least2<T>(lo[c], w) : w;
-        hi[c] = i ? most2<T>(hi[c], w) : w;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const uint64_t all = __shfl_sync(0xffffffffu, upto, 31);
+    for (; item < before + all; item += stride) {
+      const uint64_t at = item - before;
+      const int of = __popc(__ballot_sync(0xffffffffu, upto <= at));    // the sequence that holds it
+      const uint64_t in = at - (__shfl_sync(0xffffffffu, upto, of) - __shfl_sync(0xffffffffu, count, of));
+      const uint32_t entries = __shfl_sync(0xffffffffu, n, of);
+      const uint32_t logical = __shfl_sync(0xffffffffu, page0, of) + (uint32_t)(in / v.kv_heads), h = (uint32_t)(in % v.kv_heads);
+      const uint32_t page = v.table[(size_t)(s0 + of) * v.table_stride + logical];
+      if (page >= v.pages) {
+        if (lane == 0) note(v, FZ_PAGED_BAD_PAGE);
+        continue;
+      }
+      const uint32_t slots = min(v.page_slots, entries - logical * v.page_slots);
+      const uint16_t* k = v.keys + element(v, page, 0, h) + part * 8;
+      // (Slots past the page's held ones repeat its first.)
+      uint4 lo = *reinterpret_cast<const uint4*>(k), hi = lo;
+      for (uint32_t i = sub; i < slots; i += ROWS * AHEAD) {
+        uint4 x[AHEAD];
+#pragma unroll
+        for (int c = 0; c < AHEAD; c++) {
+          const uint32_t j = i + c * ROWS;
+          x[c] = __ldcs(reinterpret_cast<const uint4*>(k + (j < slots ? j : 0u) * v.slot_stride));
+        }
+#pragma unroll
+        for (int c = 0; c < AHEAD; c++) {
+          lo = make_uint4(least2<T>(lo.x, x[c].x), least2<T>(lo.y, x[c].y), least2<T>(lo.z, x[c].z), least2<T>(lo.w, x[c].w));
+          hi = make_uint4(most2<T>(hi.x, x[c].x), most2<T>(hi.y, x[c].y), most2<T>(hi.z, x[c].z), most2<T>(hi.w, x[c].w));
+        }
+      }
+#pragma unroll
+      for (int o = LANES; o < 32; o <<= 1) {
+        const uint4 l = make_uint4(__shfl_xor_sync(0xffffffffu, lo.x, o), __shfl_xor_sync(0xffffffffu, lo.y, o),
+                                   __shfl_xor_sync(0xffffffffu, lo.z, o), __shfl_xor_sync(0xffffffffu, lo.w, o));
+        const uint4 m = make_uint4(__shfl_xor_sync(0xffffffffu, hi.x, o), __shfl_xor_sync(0xffffffffu, hi.y, o),
+                                   __shfl_xor_sync(0xffffffffu, hi.z, o), __shfl_xor_sync(0xffffffffu, hi.w, o));
+        lo = make_uint4(least2<T>(lo.x, l.x), least2<T>(lo.y, l.y), least2<T>(lo.z, l.z), least2<T>(lo.w, l.w));
+        hi = make_uint4(most2<T>(hi.x, m.x), most2<T>(hi.y, m.y), most2<T>(hi.z, m.z), most2<T>(hi.w, m.w));
+      }
+      uint4* b = reinterpret_cast<uint4*>(v.bounds + ((size_t)page * v.kv_heads + h) * 2 * D);
+      if (sub == 0) {
+        b[part] = lo;
+        b[LANES + part] = hi;
       }
     }
-    uint32_t* b = reinterpret_cast<uint32_t*>(v.bounds + ((size_t)page * v.kv_heads + h) * 2 * D);
-#pragma unroll
-    for (int c = 0; c < P; c++) b[lane + 32 * c] = lo[c], b[D / 2 + lane + 32 * c] = hi[c];
+    before += all;
   }
 }
 
@@ -256,7 +325,11 @@ const void* pick(uint32_t type, uint32_t d) {
 }
 template <class T, int D>
 struct AppendOf {
-  static const void* fn() { return (const void*)append_kernel<T, D>; }
+  static const void* fn() { return (const void*)append_kernel<T, D, 1>; }
+};
+template <class T, int D>
+struct AppendManyOf {
+  static const void* fn() { return (const void*)append_kernel<T, D, 4>; }
 };
 template <class T, int D>
 struct BoundsOf {
@@ -293,10 +366,16 @@ extern "C" fz_status fz_paged_append(const fz_paged_kv* kv, const fz_paged_rows*
                      rows->q_out, rows->q_gain, rows->k_gain, rows->turns, rows->sequence, rows->index, rows->position};
   if ((st = paged_on_device(p, 16, "fz_paged_append"))) return st;
   a.r = *rows;
-  const uint64_t blocks = ((uint64_t)rows->rows * (rows->heads + 2ull * kv->kv_heads) + 7) / 8;
+  // Steps of a row, 256 / head_dim heads a warp: one a warp while they do not
+  // fill the GPU twice (8 warps a CTA, 4 CTAs an SM), else four.
+  const uint32_t a_step = 256 / kv->head_dim, steps = (rows->heads + 2 * kv->kv_heads + a_step - 1) / a_step;
+  const bool many = (uint64_t)rows->rows * steps > 2 * 148 * 32;
+  uint32_t warps = many ? (steps + 3) / 4 : steps;
+  const uint64_t blocks = ((uint64_t)rows->rows * warps + 7) / 8;
   if (blocks > 0x7FFFFFFFull) return paged_refuse(FZ_ERR_ARGUMENT, "too many rows");
-  void* args[] = {&a};
-  return paged_launch(pick<AppendOf>(kv->type, kv->head_dim), dim3((uint32_t)blocks), dim3(256), 0, 1, args, stream);
+  void* args[] = {&a, &warps};
+  return paged_launch(many ? pick<AppendManyOf>(kv->type, kv->head_dim) : pick<AppendOf>(kv->type, kv->head_dim),
+                      dim3((uint32_t)blocks), dim3(256), 0, 1, args, stream);
 }
 
 extern "C" fz_status fz_paged_bounds(const fz_paged_kv* kv, const uint32_t* first, void* stream) {
@@ -309,9 +388,9 @@ extern "C" fz_status fz_paged_bounds(const fz_paged_kv* kv, const uint32_t* firs
   const void* p[] = {kv->keys, kv->page_table, kv->lengths, kv->bounds, kv->error, first};
   if ((st = paged_on_device(p, 6, "fz_paged_bounds"))) return st;
   a.first = first;
-  const uint64_t blocks = ((uint64_t)kv->table_stride * kv->kv_heads + 7) / 8;
-  if (blocks > 0x7FFFFFFFull) return paged_refuse(FZ_ERR_ARGUMENT, "too many pages");
+  // At most four CTAs an SM (each warp then takes several pages).
+  const uint64_t blocks = ((uint64_t)kv->table_stride * kv->kv_heads * kv->sequences + 7) / 8;
   void* args[] = {&a};
-  return paged_launch(pick<BoundsOf>(kv->type, kv->head_dim), dim3((uint32_t)blocks, kv->sequences < 65535 ? kv->sequences : 65535),
-                      dim3(256), 0, 1, args, stream);
+  return paged_launch(pick<BoundsOf>(kv->type, kv->head_dim), dim3((uint32_t)std::min<uint64_t>(blocks, 4 * 148)), dim3(256), 0, 1,
+                      args, stream);
 }

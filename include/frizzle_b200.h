@@ -501,8 +501,8 @@ typedef struct fz_paged_kv {
 } fz_paged_kv;
 
 /* Appended rows: row r is a token of sequence[r] (NULL: sequence r), stored as
- * its entry index[r]; a row of sequence FZ_PAGED_NONE is padding and neither
- * read nor written.  Each query and key head is normed over its head_dim
+ * its entry index[r]; a row of sequence FZ_PAGED_NONE is padding, for which
+ * nothing is written.  Each query and key head is normed over its head_dim
  * values, x rsqrt(mean(x^2) + eps) gain (a NULL gain: not normed), then
  * rotated by position[r] (NULL: index[r]): values i and i + head_dim / 2 by
  * the angle 2 pi position turns[i], turns the frequencies in turns a position
