@@ -114,7 +114,7 @@ struct AppendArgs {
 // a few thousand positions), its fraction's sine and cosine in f32.  4,095 rows
 // of 8 + 2 + 2 heads of 256: 92 MB.
 template <class T, int D, int PASSES>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a, uint32_t warps_a_row) {
+__global__ void __launch_bounds__(128) append_kernel(const AppendArgs a, uint32_t warps_a_row) {
   constexpr int LANES = D / 8, HEADS = 32 / LANES;
   pdl_wait();
   pdl_launch_dependents();
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a, uint32_
   const PagedView& v = a.kv;
   const int lane = threadIdx.x & 31, part = lane % LANES;
   const uint32_t heads = r.heads + 2 * v.kv_heads;
-  const uint64_t warp = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint64_t warp = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const uint64_t row = (warp >> 32) ? warp / warps_a_row : (uint32_t)warp / warps_a_row;
   if (row >= r.rows) return;
   const uint32_t head0 = (uint32_t)(warp - row * warps_a_row) * (PASSES * HEADS) + lane / LANES;
@@ -243,8 +243,8 @@ FZ_DEV uint32_t most2<Bf16>(uint32_t a, uint32_t b) {
 // each 32 sequences are counted by one look at their lengths.  Memory bound:
 // every key is read once, 2 / page_slots of that written.
 template <class T, int D>
-__global__ void __launch_bounds__(256) bounds_kernel(const BoundsArgs a) {
-  constexpr int LANES = D / 8, ROWS = 32 / LANES, AHEAD = 8;
+__global__ void __launch_bounds__(256, 3) bounds_kernel(const BoundsArgs a) {
+  constexpr int LANES = D / 8, ROWS = 32 / LANES, AHEAD = 16;
   pdl_wait();
   pdl_launch_dependents();
   const PagedView& v = a.kv;
@@ -367,15 +367,15 @@ extern "C" fz_status fz_paged_append(const fz_paged_kv* kv, const fz_paged_rows*
   if ((st = paged_on_device(p, 16, "fz_paged_append"))) return st;
   a.r = *rows;
   // Steps of a row, 256 / head_dim heads a warp: one a warp while they do not
-  // fill the GPU twice (8 warps a CTA, 4 CTAs an SM), else four.
+  // fill the GPU twice (32 warps an SM), else four.
   const uint32_t a_step = 256 / kv->head_dim, steps = (rows->heads + 2 * kv->kv_heads + a_step - 1) / a_step;
   const bool many = (uint64_t)rows->rows * steps > 2 * 148 * 32;
   uint32_t warps = many ? (steps + 3) / 4 : steps;
-  const uint64_t blocks = ((uint64_t)rows->rows * warps + 7) / 8;
+  const uint64_t blocks = ((uint64_t)rows->rows * warps + 3) / 4;
   if (blocks > 0x7FFFFFFFull) return paged_refuse(FZ_ERR_ARGUMENT, "too many rows");
   void* args[] = {&a, &warps};
   return paged_launch(many ? pick<AppendManyOf>(kv->type, kv->head_dim) : pick<AppendOf>(kv->type, kv->head_dim),
-                      dim3((uint32_t)blocks), dim3(256), 0, 1, args, stream);
+                      dim3((uint32_t)blocks), dim3(128), 0, 1, args, stream);
 }
 
 extern "C" fz_status fz_paged_bounds(const fz_paged_kv* kv, const uint32_t* first, void* stream) {
@@ -388,9 +388,9 @@ extern "C" fz_status fz_paged_bounds(const fz_paged_kv* kv, const uint32_t* firs
   const void* p[] = {kv->keys, kv->page_table, kv->lengths, kv->bounds, kv->error, first};
   if ((st = paged_on_device(p, 6, "fz_paged_bounds"))) return st;
   a.first = first;
-  // At most four CTAs an SM (each warp then takes several pages).
+  // At most three CTAs an SM (each warp then takes several pages).
   const uint64_t blocks = ((uint64_t)kv->table_stride * kv->kv_heads * kv->sequences + 7) / 8;
   void* args[] = {&a};
-  return paged_launch(pick<BoundsOf>(kv->type, kv->head_dim), dim3((uint32_t)std::min<uint64_t>(blocks, 4 * 148)), dim3(256), 0, 1,
+  return paged_launch(pick<BoundsOf>(kv->type, kv->head_dim), dim3((uint32_t)std::min<uint64_t>(blocks, 3 * 148)), dim3(256), 0, 1,
                       args, stream);
 }
