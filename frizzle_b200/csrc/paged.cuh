@@ -59,6 +59,50 @@ FZ_DEV uint64_t element(const PagedView& v, uint32_t page, uint32_t slot, uint32
   return page * v.page_stride + slot * v.slot_stride + head * v.head_stride;
 }
 
+// 16-byte copies into shared memory (zeros where not valid), by groups.
+FZ_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+FZ_DEV void copy16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+FZ_DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+FZ_DEV void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <class T>
+FZ_DEV void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (T::kType == FZ_KV_F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A pair of f32 as pairs of the cache's type that sum to it: f16 part and
+// remainder (22 bits), the remainder times `lift`; bf16 three parts (24 bits).
+template <class T>
+struct Parts {
+  static constexpr int N = T::kType == FZ_KV_F16 ? 2 : 3;
+  uint32_t w[4];
+};
+template <class T>
+FZ_DEV Parts<T> parts(float x, float y, float lift = 1.f) {
+  Parts<T> p;
+#pragma unroll
+  for (int i = 0; i < Parts<T>::N; i++) {
+    p.w[i] = T::pack(x, y);
+    const float2 u = T::unpack(p.w[i]);
+    x = (x - u.x) * lift, y = (y - u.y) * lift;
+  }
+#pragma unroll
+  for (int i = Parts<T>::N; i < 4; i++) p.w[i] = 0;
+  return p;
+}
+
 // ------------------------------------------------------------ host side
 
 // FZ_OK, or the refusal (its message set) of a cache description; `need` are

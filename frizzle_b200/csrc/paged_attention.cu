@@ -207,15 +207,6 @@ FZ_DEV Walk begin(const Share& sh, uint32_t unit) {
   return Walk{sh.s, sh.h, (sh.l.count + unit - 1) / unit, sh.at, 0, sh.l};
 }
 
-FZ_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-FZ_DEV void copy16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-FZ_DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-FZ_DEV void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 FZ_DEV void matrices(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -229,39 +220,6 @@ FZ_DEV uint32_t transpose(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-template <class T>
-FZ_DEV void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if (T::kType == FZ_KV_F16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// A pair of f32 as pairs of the cache's type that sum to it: f16 part and
-// remainder (22 bits), the remainder times `lift`; bf16 three parts (24 bits).
-template <class T>
-struct Parts {
-  static constexpr int N = T::kType == FZ_KV_F16 ? 2 : 3;
-  uint32_t w[4];
-};
-template <class T>
-FZ_DEV Parts<T> parts(float x, float y, float lift = 1.f) {
-  Parts<T> p;
-#pragma unroll
-  for (int i = 0; i < Parts<T>::N; i++) {
-    p.w[i] = T::pack(x, y);
-    const float2 u = T::unpack(p.w[i]);
-    x = (x - u.x) * lift, y = (y - u.y) * lift;
-  }
-#pragma unroll
-  for (int i = Parts<T>::N; i < 4; i++) p.w[i] = 0;
-  return p;
-}
-
 // exp2 of a difference to the maximum of `m`'s side: 0 for a side without entries.
 FZ_DEV float fold(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
 

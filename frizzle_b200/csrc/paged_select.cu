@@ -23,6 +23,9 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kBins = 2048;           // 11 bits a digit
 constexpr int kMaxCluster = 8;
+constexpr uint32_t kNear = 256;       // pages near a threshold that the first CTA scores in f64
+constexpr uint32_t kStages = 4;       // stages of 64 bytes of 32 rows in a warp's shared memory
+constexpr size_t kRing = kThreads / 32 * kStages * 4 * 32 * 16;
 
 // A CTA's shared memory in a cluster.  What CTAs tell one another they write
 // into all the others' boxes before a cluster barrier, so that after it every
@@ -38,12 +41,25 @@ struct Shared {
   uint2 taken[kMaxCluster];           // its keys above the threshold, and equal to it
   uint2 zones[kMaxCluster];           // its pages surely in, and near the threshold
   float bound[kMaxCluster];           // its greatest |bound|
+  float4 verdict;                     // the first CTA's choice: whether to refine, and the zones' ends
 };
+// The CTAs that choose together: a cluster, or one CTA alone.
+struct Group {
+  cg::cluster_group* cluster;
+  uint32_t size, rank;
+};
+FZ_DEV void sync(const Group& g) {
+  if (g.cluster) g.cluster->sync();
+  else __syncthreads();
+}
+template <class V>
+FZ_DEV V* theirs(const Group& g, V* mine, uint32_t c) {
+  return g.cluster ? g.cluster->map_shared_rank(mine, c) : mine;
+}
 // `value` into the box of this CTA's rank in every CTA; by the first warp.
 template <class V>
-FZ_DEV void tell(cg::cluster_group& cluster, V* boxes, V value) {
-  const uint32_t c = threadIdx.x;
-  if (c < cluster.num_blocks()) *cluster.map_shared_rank(boxes + cluster.block_rank(), c) = value;
+FZ_DEV void tell(const Group& g, V* boxes, V value) {
+  if (threadIdx.x < g.size) *theirs(g, boxes + g.rank, threadIdx.x) = value;
 }
 
 // Order-preserving unsigned keys, -0 as +0, every NaN above +inf; 0 is no key.
@@ -91,9 +107,9 @@ struct Threshold {
 // highest bit in which the keys differ, so that scores of like size take one
 // or two.
 template <class K, class Forced>
-FZ_DEV Threshold<K> find(cg::cluster_group& cluster, Shared& sh, const K* keys, uint32_t n, uint32_t first, uint32_t take,
+FZ_DEV Threshold<K> find(const Group& group, Shared& sh, const K* keys, uint32_t n, uint32_t first, uint32_t take,
                          Forced forced) {
-  const uint32_t size = cluster.num_blocks();
+  const uint32_t size = group.size;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   Threshold<K> r{0, 0, 0, 0, false, false};
   // How many are free, and the bits in which they differ.
@@ -127,10 +143,10 @@ FZ_DEV Threshold<K> find(cg::cluster_group& cluster, Shared& sh, const K* keys, 
       a = x < a ? x : a;
       b = y > b ? y : b;
     }
-    tell(cluster, sh.count, make_uint4(n, p, 0, 0));
-    tell(cluster, sh.span, make_ulonglong2(a, b));
+    tell(group, sh.count, make_uint4(n, p, 0, 0));
+    tell(group, sh.span, make_ulonglong2(a, b));
   }
-  cluster.sync();
+  sync(group);
   uint32_t all = 0, all_pinned = 0;
   least = ~(K)0, most = 0;
   for (uint32_t c = 0; c < size; c++) {
@@ -160,15 +176,15 @@ FZ_DEV Threshold<K> find(cg::cluster_group& cluster, Shared& sh, const K* keys, 
       const K k = keys[i];
       if ((k & r.mask) == r.prefix && !forced(first + i)) atomicAdd(&sh.bins[(uint32_t)(k >> shift) & digits], 1u);
     }
-    cluster.sync();
-    if (cluster.block_rank() == 0) {
+    sync(group);
+    if (group.rank == 0) {
       // Thread t: four bins from the top, summed over the cluster.
       const uint32_t at = kBins / 4 - 1 - t;
       uint4 sum = make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (uint32_t c = 0; c < kMaxCluster; c++)
         if (c < size) {
-          const uint4 b = reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.bins, c))[at];
+          const uint4 b = reinterpret_cast<const uint4*>(theirs(group, sh.bins, c))[at];
           sum.x += b.x, sum.y += b.y, sum.z += b.z, sum.w += b.w;
         }
       const uint32_t count[4] = {sum.w, sum.z, sum.y, sum.x};
@@ -177,11 +193,11 @@ FZ_DEV Threshold<K> find(cg::cluster_group& cluster, Shared& sh, const K* keys, 
       for (uint32_t i = 0; i < 4; i++) {
         if (before < want && want <= before + count[i])
           for (uint32_t c = 0; c < size; c++)
-            *cluster.map_shared_rank(&sh.step, c) = make_uint4(4 * at + 3 - i, before, count[i], 0);
+            *theirs(group, &sh.step, c) = make_uint4(4 * at + 3 - i, before, count[i], 0);
         before += count[i];
       }
     }
-    cluster.sync();
+    sync(group);
     const uint4 step = sh.step;
     for (uint32_t i = t; i < kBins / 4; i += kThreads) reinterpret_cast<uint4*>(sh.bins)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
@@ -195,21 +211,98 @@ FZ_DEV Threshold<K> find(cg::cluster_group& cluster, Shared& sh, const K* keys, 
   return r;
 }
 
+// The same by one CTA with all the keys: 8 bits a digit, their 256 bins summed by
+// one warp, so that a digit costs two barriers and little else.
+template <class Forced>
+FZ_DEV Threshold<uint32_t> find_alone(Shared& sh, const uint32_t* keys, uint32_t n, uint32_t take, Forced forced) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  Threshold<uint32_t> r{0, 0, 0, 0, false, false};
+  uint32_t pinned = 0, least = ~0u, most = 0;
+  for (uint32_t i = t; i < n; i += kThreads) {
+    const uint32_t k = keys[i];
+    if (forced(i)) pinned++;
+    else least = min(least, k), most = max(most, k);
+  }
+  pinned = __reduce_add_sync(0xffffffffu, pinned);
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) sh.warp[0][warp] = pinned, sh.range[0][warp] = least, sh.range[1][warp] = most;
+  for (int i = t; i < 4 * 256; i += kThreads) sh.bins[i] = 0;
+  __syncthreads();
+  pinned = 0, least = ~0u, most = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; w++) {
+    pinned += sh.warp[0][w];
+    least = min(least, (uint32_t)sh.range[0][w]);
+    most = max(most, (uint32_t)sh.range[1][w]);
+  }
+  uint32_t want = take > pinned ? take - pinned : 0u;
+  r.want = r.ties = want;
+  if (want >= n - pinned) {
+    r.every = true, r.ties = n - pinned;
+    return r;
+  }
+  if (!want) {
+    r.none = true;
+    return r;
+  }
+  int high = least == most ? 0 : 32 - __clz((int)(least ^ most));
+  r.mask = high == 32 ? 0u : ~0u << high;
+  r.prefix = most & r.mask;
+  for (uint32_t* bins = sh.bins; high > 0; bins += 256) {
+    const int bits = high < 8 ? high : 8, shift = high - bits;
+    const uint32_t digits = (1u << bits) - 1;
+    for (uint32_t i = t; i < n; i += kThreads) {
+      const uint32_t k = keys[i];
+      if ((k & r.mask) == r.prefix && !forced(i)) atomicAdd(&bins[(k >> shift) & digits], 1u);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      // Lane l: eight bins from the top.
+      uint32_t count[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) count[i] = bins[255 - (8 * lane + i)], sum += count[i];
+      uint32_t upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      uint32_t before = upto - sum;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        if (before < want && want <= before + count[i]) sh.step = make_uint4(255 - (8 * lane + i), before, count[i], 0);
+        before += count[i];
+      }
+    }
+    __syncthreads();
+    const uint4 step = sh.step;
+    want -= step.y;
+    r.prefix |= step.x << shift;
+    r.mask |= digits << shift;
+    r.ties = want;
+    high = shift;
+    if (want == step.z) break;           // the digit's keys are all taken
+  }
+  return r;
+}
+
 // emit(i, taken, rank) for every entry i of the CTA's n, the taken ones ranked in
 // ascending order over the cluster: state(i) 2 taken, 1 a tie, of which the cluster's first `ties`
 // are taken, 0 not.  Each thread takes a run of the slice.
 template <class State, class Emit>
-FZ_DEV void emit_taken(cg::cluster_group& cluster, Shared& sh, uint32_t n, uint32_t ties, State state, Emit emit) {
-  const uint32_t rank = cluster.block_rank(), run = (n + kThreads - 1) / kThreads;
+FZ_DEV void emit_taken(const Group& group, Shared& sh, uint32_t n, uint32_t ties, State state, Emit emit) {
+  const uint32_t rank = group.rank, run = (n + kThreads - 1) / kThreads;
   const uint32_t i0 = min(n, threadIdx.x * run), i1 = min(n, i0 + run);
+  __syncthreads();                       // (sh.warp is read)
   uint2 mine = make_uint2(0, 0);
   for (uint32_t i = i0; i < i1; i++) {
     const int s = state(i);
     mine.x += s == 2, mine.y += s == 1;
   }
   uint2 at = block_scan(sh, mine);
-  if (threadIdx.x < 32) tell(cluster, sh.taken, make_uint2(sh.more, sh.equal));
-  cluster.sync();                        // (its arrival is the last thing a CTA does in another's shared memory)
+  if (threadIdx.x < 32) tell(group, sh.taken, make_uint2(sh.more, sh.equal));
+  sync(group);                        // (its arrival is the last thing a CTA does in another's shared memory)
   for (uint32_t c = 0; c < rank; c++) at.x += sh.taken[c].x, at.y += sh.taken[c].y;
   for (uint32_t i = i0; i < i1; i++) {
     const int s = state(i);
@@ -264,194 +357,323 @@ FZ_DEV double page_score(const SelectArgs& a, const float* q, uint32_t page, uin
   return best;
 }
 
-// The scores are wanted in 64 bits, and 64-bit conversions run at an eighth of
-// the rate of f32 arithmetic or less, so they are made for few pages only.
-// First every page's score in f32, off by at most
-//   E = 16 x 2^-24 x max_g sum |q| x max |bound|
-// (8 fused products a lane and 5 sums over lanes, each within 2^-24 of the sum
-// of the products' sizes), and the threshold T among those.  The take-th
-// largest true score is then within E of T: pages more than 2 E above T are in,
-// pages more than 2 E below are out, and only where more pages lie in between
-// than are wanted are those scored in f64 and chosen among by that.  With a
-// score or a bound that is not finite, E is not either, and every page is.
+template <class T>
+FZ_DEV uint32_t greater_size(uint32_t m, uint32_t x);
+template <>
+FZ_DEV uint32_t greater_size<F16>(uint32_t m, uint32_t x) {
+  const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&m), __habs2(*reinterpret_cast<__half2*>(&x)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <>
+FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
+  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&m), __habs2(*reinterpret_cast<__nv_bfloat162*>(&x)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// The choice is wanted by the scores in 64 bits, and 64-bit conversions run at an
+// eighth of the rate of f32 arithmetic or less, so those are made for few pages
+// only.  First every page's score to f32 accuracy, off by at most
+//   E = (80 x 2^-24 + 2^-21) x (max_g sum |q| + D / 8 max |q|) x max |bound|
+// (below), and the threshold T among those.  The take-th largest true score is
+// then within E of T: pages more than 2 E above T are in, pages more than 2 E
+// below are out, and only where more pages lie in between than are wanted are
+// those scored in f64 and chosen among by that (a page or two of two thousand,
+// as a rule).  With a score or a bound that is not finite, E is not either, and
+// every page is.
 //
-// f32: D / 8 lanes a page, 8 dimensions a lane, four pages at a time, their
-// loads first, each head's q from shared memory once for the four; their sums
-// over the lanes are halved page by page (6 shuffles for four pages, not 20).
-template <class T, int D>
-__global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a, uint32_t slice) {
-  constexpr int LANES = D / 8, PW = 32 / LANES, BATCH = 4;
+// The scores are products of the pages' rows of 2 D least and greatest keys with
+// q's negative and positive parts: mma.sync m16n8k16 with 16 pages in M and the
+// heads' parts of the cache's type in N, as attend_kernel has them (f16 22 bits
+// of q, bf16 24).  The order of the 2 D products is free, so a lane takes 16
+// bytes of a row as they lie for two steps' A operands; it copies them itself,
+// by cp.async three stages ahead, and no barrier or ldmatrix comes between.  Two
+// MMAs run into one f32 sum (32 additions to at least single precision, 2^-23 of
+// the products' sizes each), those are added by f32 (2 D / 32 of them, and the
+// parts): 64 + 16 times 2^-24, and 2^-22 and the subnormal parts' 2^-25 for what
+// q's parts leave out.  f32 lanes and shuffles instead took 60 us where this
+// takes 30 (16 sequences, 4 KV heads, up to 2,048 pages: 94 MB).
+//
+// Where one CTA's shared memory holds all the cluster's scores (`together`), the
+// first CTA gets them all and chooses alone, two cluster barriers in all; beyond
+// that the cluster does digit by digit.
+template <class T, int D, int GP>
+__global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a, uint32_t slice, uint32_t together) {
+  constexpr int STEPS = D / 8, NT = (Parts<T>::N * GP + 7) / 8;        // 16-product steps a page; column tiles
+  constexpr uint32_t STAGES = D / 32;                                  // stages (4 steps) a tile of 16 pages
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Shared sh;
-  __shared__ float norm[8], bound[kThreads / 32];
-  uint64_t* exact = reinterpret_cast<uint64_t*>(dyn);                  // f64 scores of the pages in between
-  uint32_t* keys = reinterpret_cast<uint32_t*>(exact + slice);
-  float* q = reinterpret_cast<float*>(keys + slice);
+  __shared__ float norm[8], scale[8], bound[kThreads / 32];
+  __shared__ uint32_t near_at[kNear], nears;
+  __shared__ uint64_t near_key[kNear];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, t4 = lane & 3, g4 = lane >> 2;
+  // [stage][piece][lane]: what a lane copies it alone reads.
+  uint4* ring = reinterpret_cast<uint4*>(dyn) + warp * kStages * 4 * 32 + lane;
+  uint2* qf = reinterpret_cast<uint2*>(dyn + kRing);                   // [STEPS][NT][32] q's B operands
+  uint64_t* exact = reinterpret_cast<uint64_t*>(qf + STEPS * NT * 32); // f64 scores of the pages in between
+  uint32_t* keys = reinterpret_cast<uint32_t*>(exact + slice);         // this CTA's, in the first CTA all with `together`
+  uint32_t* chosen = keys + (together ? together : slice);             // a bit a page: near the threshold and taken
   cg::cluster_group cluster = cg::this_cluster();
   cluster.barrier_arrive();                        // (waited for before the first word to another CTA)
   pdl_wait();
   pdl_launch_dependents();
   const PagedView& v = a.kv;
-  const uint32_t size = cluster.num_blocks(), rank = cluster.block_rank();
+  const uint32_t size = cluster.num_blocks(), rank = cluster.block_rank(), G = a.group;
+  const Group whole{&cluster, size, rank}, single{nullptr, 1, 0};
   const uint64_t item = blockIdx.x / size;
   const uint32_t s = (uint32_t)(item / v.kv_heads), h = (uint32_t)(item % v.kv_heads);
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const float4* q4 = reinterpret_cast<const float4*>(a.q + s * a.q_stride + (size_t)h * a.group * D);
-  for (uint32_t i = t; i < a.group * D / 4; i += kThreads) reinterpret_cast<float4*>(q)[i] = __ldcg(q4 + i);
+  const float* q = a.q + s * a.q_stride + (size_t)h * G * D;
   const uint32_t entries = held(v, s);
   if (t == 0 && rank == 0 && v.lengths[s] > entries) note(v, FZ_PAGED_BAD_LENGTH);
   const uint32_t pages = (entries + v.page_slots - 1) / v.page_slots;
+  const uint32_t per = (pages + size - 1) / size, first = min(pages, rank * per), n = min(pages, first + per) - first;
+  const uint32_t* table = v.table + (size_t)s * v.table_stride;
+
+  // The copies, kStages - 1 stages ahead of their use: rows g4 and g4 + 8 of the
+  // tile, 16 bytes of every 64.
+  auto look = [&](uint32_t tile) {
+    const uint32_t i = tile * 16 + lane;
+    return lane < 16 && i < n ? table[first + i] : FZ_PAGED_NONE;
+  };
+  uint32_t ahead = warp, word = look(warp);
+  const uint4 *row0 = nullptr, *row1 = nullptr;
+  bool ok0 = false, ok1 = false;
+  uint32_t fetched = 0;
+  auto fetch = [&]() {
+    const uint32_t st = fetched % STAGES;
+    if (st == 0) {
+      const uint32_t p0 = __shfl_sync(0xffffffffu, word, g4), p1 = __shfl_sync(0xffffffffu, word, g4 + 8);
+      ok0 = p0 < v.pages, ok1 = p1 < v.pages;
+      const uint4* b = reinterpret_cast<const uint4*>(v.bounds);
+      row0 = b + ((size_t)(ok0 ? p0 : 0u) * v.kv_heads + h) * (D / 4) + t4;
+      row1 = b + ((size_t)(ok1 ? p1 : 0u) * v.kv_heads + h) * (D / 4) + t4;
+      ahead += kThreads / 32;
+      word = look(ahead);
+    }
+    const uint32_t slot = smem_u32(ring + (fetched % kStages) * 4 * 32);
+    copy16(slot, row0 + 8 * st, ok0);
+    copy16(slot + 512, row1 + 8 * st, ok1);
+    copy16(slot + 1024, row0 + 8 * st + 4, ok0);
+    copy16(slot + 1536, row1 + 8 * st + 4, ok1);
+    copy_commit();
+    fetched++;
+  };
+#pragma unroll
+  for (uint32_t k = 0; k < kStages - 1; k++) fetch();
+
   uint32_t* out = a.blocks + item * a.top;
   float* scores = a.scores ? a.scores + item * a.top : nullptr;
   for (uint32_t i = min(pages, a.top) + rank * kThreads + t; i < a.top; i += size * kThreads) {
     out[i] = FZ_PAGED_NONE;
     if (scores) scores[i] = 0.f;
   }
-  const uint32_t per = (pages + size - 1) / size, first = min(pages, rank * per), n = min(pages, first + per) - first;
-  const uint32_t* table = v.table + (size_t)s * v.table_stride + first;
+  // q: each head's size and scale (the largest to [1, 2)), then its parts.
+  if (warp < GP) {
+    float sum = 0.f, top = 0.f;
+    for (int i = lane; i < D / 4 && warp < (int)G; i += 32) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(q + warp * D) + i);
+      sum += fabsf(x.x) + fabsf(x.y) + fabsf(x.z) + fabsf(x.w);
+      top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+    }
+    sum = warp_sum(sum), top = warp_max(top);
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);   // 2^(e - 127) <= top
+    if (lane == 0) norm[warp] = sum + top * (D / 8), scale[warp] = top == INFINITY ? NAN : __uint_as_float((uint32_t)e << 23);
+  }
   __syncthreads();
-  if (warp < (int)a.group) {
-    float x = 0.f;
-    for (int i = lane; i < D; i += 32) x += fabsf(q[warp * D + i]);
-    x = warp_sum(x);
-    if (lane == 0) norm[warp] = x;
+  {
+    const uint32_t g = g4 % GP;
+    const float down = __uint_as_float((254u << 23) - __float_as_uint(scale[g]));   // the reciprocal of a power of two
+    for (int k = warp; k < STEPS; k += kThreads / 32) {
+      const int at = ((k / 2) * 4 + t4) * 8 + (k & 1) * 4;              // of the row's 2 D: least keys, then greatest
+      const float4 x = g < G ? __ldcg(reinterpret_cast<const float4*>(q + g * D + at % D)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      // (a NaN stays one in both)
+      const bool least = at < D;
+      const float y[4] = {(x.x < 0.f) == least ? x.x : x.x * 0.f, (x.y < 0.f) == least ? x.y : x.y * 0.f,
+                          (x.z < 0.f) == least ? x.z : x.z * 0.f, (x.w < 0.f) == least ? x.w : x.w * 0.f};
+      const Parts<T> p0 = parts<T>(y[0] * down, y[1] * down), p1 = parts<T>(y[2] * down, y[3] * down);
+#pragma unroll
+      for (int c = 0; c < NT; c++)
+        qf[(k * NT + c) * 32 + lane] = GP == 8 ? make_uint2(p0.w[c], p1.w[c])
+                                               : (g4 < 4 ? make_uint2(p0.w[2 * c], p1.w[2 * c])
+                                                         : make_uint2(p0.w[2 * c + 1], p1.w[2 * c + 1]));
+    }
   }
+  __syncthreads();
 
-  // Every page in f32.
-  const int part = lane % LANES, sub = lane / LANES;
-  float largest = 0.f;
-  constexpr uint32_t STEP = kThreads / 32 * BATCH * PW;
-  uint32_t base = warp * BATCH * PW;
-  uint32_t word = lane < BATCH * PW && base + lane < n ? table[base + lane] : FZ_PAGED_NONE;
-  for (; base < n; base += STEP) {
-    uint4 lo[BATCH], hi[BATCH];
-    uint32_t page[BATCH];
+  // Every page to f32 accuracy.
+  uint32_t largest = 0, used = 0;
+  const float c0 = scale[(2 * t4) % GP], c1 = scale[(2 * t4 + 1) % GP];
+  const bool has0 = (2 * t4) % GP < G, has1 = (2 * t4 + 1) % GP < G;
+  for (uint32_t tile = warp; tile * 16 < n; tile += kThreads / 32) {
+    const uint32_t mine = look(tile);
+    float sum[NT][4];
 #pragma unroll
-    for (int p = 0; p < BATCH; p++) {
-      page[p] = __shfl_sync(0xffffffffu, word, p * PW + sub);
-      const uint4* b = reinterpret_cast<const uint4*>(v.bounds + ((size_t)(page[p] < v.pages ? page[p] : 0u) * v.kv_heads + h) * 2 * D);
-      lo[p] = __ldcg(b + part);
-      hi[p] = __ldcg(b + LANES + part);
-    }
-    word = lane < BATCH * PW && base + STEP + lane < n ? table[base + STEP + lane] : FZ_PAGED_NONE;
-    float x[BATCH][8], y[BATCH][8], best[BATCH];
+    for (int c = 0; c < NT; c++)
 #pragma unroll
-    for (int p = 0; p < BATCH; p++) {
-      const uint32_t l[4] = {lo[p].x, lo[p].y, lo[p].z, lo[p].w}, u[4] = {hi[p].x, hi[p].y, hi[p].z, hi[p].w};
+      for (int i = 0; i < 4; i++) sum[c][i] = 0.f;
+#pragma unroll 1
+    for (uint32_t st = 0; st < STAGES; st++, used++) {
+      copy_wait<kStages - 2>();
+      const uint4* at = ring + (used % kStages) * 4 * 32;
+      const uint4 r0 = at[0], r1 = at[32], r2 = at[64], r3 = at[96];
+      fetch();
+      const uint32_t words[16] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w, r2.x, r2.y, r2.z, r2.w, r3.x, r3.y, r3.z, r3.w};
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float2 f = T::unpack(l[i]), g = T::unpack(u[i]);
-        x[p][2 * i] = f.x, x[p][2 * i + 1] = f.y, y[p][2 * i] = g.x, y[p][2 * i + 1] = g.y;
-        if (page[p] < v.pages) largest = fmaxf(largest, fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(g.x), fabsf(g.y))));
+      for (int i = 0; i < 16; i++) largest = greater_size<T>(largest, words[i]);
+      const uint32_t a0[4] = {r0.x, r1.x, r0.y, r1.y}, a1[4] = {r0.z, r1.z, r0.w, r1.w};
+      const uint32_t a2[4] = {r2.x, r3.x, r2.y, r3.y}, a3[4] = {r2.z, r3.z, r2.w, r3.w};
+#pragma unroll
+      for (int c = 0; c < NT; c++) {
+        const uint2* b = qf + (st * 4 * NT + c) * 32 + lane;
+        const uint2 b0 = b[0], b1 = b[NT * 32], b2 = b[2 * NT * 32], b3 = b[3 * NT * 32];
+        float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+        mma<T>(x, a0, b0.x, b0.y);
+        mma<T>(y, a2, b2.x, b2.y);
+        mma<T>(x, a1, b1.x, b1.y);
+        mma<T>(y, a3, b3.x, b3.y);
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[c][i] += x[i] + y[i];
       }
-      best[p] = -INFINITY;
     }
-    float top = 0.f;
-    const bool half = lane & (LANES / 2), quarter = lane & (LANES / 4);
-    for (uint32_t g = 0; g < a.group; g++) {
-      const float4 qa = reinterpret_cast<const float4*>(q + g * D)[2 * part], qb = reinterpret_cast<const float4*>(q + g * D)[2 * part + 1];
-      const float qs[8] = {qa.x, qa.y, qa.z, qa.w, qb.x, qb.y, qb.z, qb.w};
-      float sum[BATCH] = {0.f, 0.f, 0.f, 0.f};
+    // Rows g4 and g4 + 8, columns 2 t4 and 2 t4 + 1: the heads' parts together, the largest of the heads.
+    uint32_t best[2];
 #pragma unroll
-      for (int i = 0; i < 8; i++)
+    for (int r = 0; r < 2; r++) {
+      float x = sum[0][2 * r], y = sum[0][2 * r + 1];
 #pragma unroll
-        for (int p = 0; p < BATCH; p++) sum[p] = fmaf(qs[i], qs[i] < 0.f ? x[p][i] : y[p][i], sum[p]);
-      // (a lane's page is 2 half + quarter from here on)
-      const float u0 = (half ? sum[2] : sum[0]) + __shfl_xor_sync(0xffffffffu, half ? sum[0] : sum[2], LANES / 2);
-      const float u1 = (half ? sum[3] : sum[1]) + __shfl_xor_sync(0xffffffffu, half ? sum[1] : sum[3], LANES / 2);
-      float u = (quarter ? u1 : u0) + __shfl_xor_sync(0xffffffffu, quarter ? u0 : u1, LANES / 4);
-#pragma unroll
-      for (int o = LANES / 8; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-      top = g == 0 || order(u) > order(top) ? u : top;
-    }
-    const int p = (half ? 2 : 0) + (quarter ? 1 : 0);
-    const uint32_t i = base + p * PW + sub;
-    const bool ok = (p == 0 ? page[0] : p == 1 ? page[1] : p == 2 ? page[2] : page[3]) < v.pages;
-    if (part % (LANES / 4) == 0 && i < n) {
-      keys[i] = ok ? order(top) : 0u;
-      if (!ok) note(v, FZ_PAGED_BAD_PAGE);
+      for (int c = 1; c < NT; c++) x += sum[c][2 * r], y += sum[c][2 * r + 1];
+      if (GP == 4) x += __shfl_xor_sync(0xffffffffu, x, 2), y += __shfl_xor_sync(0xffffffffu, y, 2);
+      best[r] = max(has0 ? order(x * c0) : 0u, has1 ? order(y * c1) : 0u);
+      best[r] = max(best[r], __shfl_xor_sync(0xffffffffu, best[r], 1));
+      if (GP == 8) best[r] = max(best[r], __shfl_xor_sync(0xffffffffu, best[r], 2));
+      const uint32_t i = tile * 16 + g4 + 8 * r, page = __shfl_sync(0xffffffffu, mine, g4 + 8 * r);
+      if (t4 == 0 && i < n) {
+        keys[i] = page < v.pages ? best[r] : 0u;
+        if (page >= v.pages) note(v, FZ_PAGED_BAD_PAGE);
+      }
     }
   }
-  largest = warp_max(largest);
-  if (lane == 0) bound[warp] = largest;
+  copy_wait<0>();
+  const float2 sizes = T::unpack(largest);
+  const float warp_largest = warp_max(fmaxf(sizes.x, sizes.y));
+  if (lane == 0) bound[warp] = warp_largest;
   __syncthreads();
   cluster.barrier_wait();
-  if (warp == 0) {
-    for (int w = 1; w < kThreads / 32; w++) largest = fmaxf(largest, bound[w]);
-    tell(cluster, sh.bound, largest);
+  if (warp == 0) tell(whole, sh.bound, warp_max(lane < kThreads / 32 ? bound[lane] : 0.f));
+  const bool alone = together && size > 1;
+  if (alone && rank) {
+    uint32_t* all = cluster.map_shared_rank(keys, 0) + first;
+    for (uint32_t i = t; i < n; i += kThreads) all[i] = keys[i];
   }
+  if (alone) cluster.sync();
+  else __syncthreads();
 
-  // The threshold among them (its first barrier makes the bounds seen).  A free page's zone: 2 in, 1 near T, 0 out.
+  // The threshold among them, by the first CTA alone or by all (their first
+  // barrier makes the bounds seen).  A free page's zone: 2 in, 1 near T, 0 out.
+  const bool one = alone || size == 1;
   const uint32_t take = min(a.top, pages);
   auto forced = [&](uint32_t i) { return i < a.sink || i + a.recent >= pages; };
-  const Threshold<uint32_t> r = find(cluster, sh, keys, n, first, take, forced);
-  bool refine = false;
+  bool refine = false;                             // too many near T for the first CTA: all of them score theirs in f64
+  Threshold<uint32_t> r{};
   float above = 0.f, below = 0.f;
+  bool vague = false;                              // E is not finite: every page is near
   auto zone = [&](uint32_t key) {
     const float x = __uint_as_float(topk_bits(key));
-    return key == 0u || x < below ? 0 : x > above || x != x ? 2 : 1;
+    return key == 0u ? 0 : vague ? 1 : x < below ? 0 : x > above || x != x ? 2 : 1;
   };
-  if (!r.every && !r.none) {
-    float m = 0.f, norms = 0.f;
-    for (uint32_t c = 0; c < size; c++) m = fmaxf(m, sh.bound[c]);
-    for (uint32_t g = 0; g < a.group; g++) norms = norm[g] > norms || norm[g] != norm[g] ? norm[g] : norms;
-    const float e = 2.f * 16.f * 5.9604645e-8f * norms * m;
-    const uint32_t low = r.prefix, high = r.prefix | ~r.mask;
-    // The ends' scores, as topk_key orders them.  (A NaN threshold: ties by the index, as in f64.)
-    const float tl = __uint_as_float(topk_bits(low)), th = __uint_as_float(topk_bits(high));
-    below = tl - e, above = th == th ? th + e : INFINITY;
-    uint32_t in = 0, near = 0;
-    for (uint32_t i = t; i < n; i += kThreads) {
-      const int z = forced(first + i) ? 0 : zone(keys[i]);
-      in += z == 2, near += z == 1;
-    }
-    in = __reduce_add_sync(0xffffffffu, in), near = __reduce_add_sync(0xffffffffu, near);
-    __syncthreads();
-    if (lane == 0) sh.warp[0][warp] = in, sh.warp[1][warp] = near;
-    __syncthreads();
-    if (warp == 0) {
-      in = lane < kThreads / 32 ? sh.warp[0][lane] : 0u, near = lane < kThreads / 32 ? sh.warp[1][lane] : 0u;
+  if (!alone || rank == 0) {
+    const Group group = one ? single : whole;
+    const uint32_t from = one ? 0u : first, count = one ? pages : n;
+    r = one ? find_alone(sh, keys, count, take, forced) : find(group, sh, keys, count, from, take, forced);
+    bool by_bit = false;
+    if (!r.every && !r.none) {
+      float m = 0.f, norms = 0.f;
+      for (uint32_t c = 0; c < size; c++) m = fmaxf(m, sh.bound[c]);
+      for (uint32_t g = 0; g < G; g++) norms = norm[g] > norms || norm[g] != norm[g] ? norm[g] : norms;
+      const float e = 2.f * (80.f + 8.f) * 5.9604645e-8f * norms * m;
+      // The ends' scores, as topk_key orders them.  (A NaN threshold: ties by the index, as in f64.)
+      const float tl = __uint_as_float(topk_bits(r.prefix)), th = __uint_as_float(topk_bits(r.prefix | ~r.mask));
+      below = tl - e, above = th == th ? th + e : INFINITY, vague = !(e < INFINITY);
+      uint32_t in = 0, near = 0;
+      if (t == 0) nears = 0;
+      for (uint32_t i = t; i < count; i += kThreads) {
+        const int z = forced(from + i) ? 0 : zone(keys[i]);
+        in += z == 2, near += z == 1;
+      }
       in = __reduce_add_sync(0xffffffffu, in), near = __reduce_add_sync(0xffffffffu, near);
-      tell(cluster, sh.zones, make_uint2(in, near));
-    }
-    cluster.sync();
-    in = near = 0;
-    for (uint32_t c = 0; c < size; c++) in += sh.zones[c].x, near += sh.zones[c].y;
-    refine = tl == tl && in + near != r.want;
-  }
-  Threshold<uint64_t> r64{};
-  auto taken_first = [&](uint32_t i) { return forced(i) || zone(keys[i - first]) == 2; };
-  if (refine) {
-    for (uint32_t i = warp; i < n; i += kThreads / 32) {
-      double d = 0.0;
-      const bool near = !forced(first + i) && zone(keys[i]) == 1;
-      if (near) d = page_score<T, D>(a, q, table[i], h, lane);
-      if (lane == 0) exact[i] = near ? order(d) : 0ull;
-    }
-    __syncthreads();
-    r64 = find(cluster, sh, exact, n, first, take, taken_first);
-  }
-  emit_taken(
-      cluster, sh, n, refine ? r64.ties : r.ties,
-      [&](uint32_t i) {
-        return refine ? state_of(r64, exact[i], taken_first(first + i)) : state_of(r, keys[i], forced(first + i));
-      },
-      [&](uint32_t i, bool taken, uint32_t at) {
-        if (taken) out[at] = first + i;
-        if (scores) exact[i] = taken ? at + 1 : 0;
-      });
-  if (scores) {
-    __syncthreads();
-    for (uint32_t i0 = warp * 32; i0 < n; i0 += kThreads) {
-      const uint32_t at = i0 + lane < n ? (uint32_t)exact[i0 + lane] : 0u;
-      for (uint32_t left = __ballot_sync(0xffffffffu, at != 0); left; left &= left - 1) {
-        const int l = __ffs(left) - 1;
-        const uint32_t page = table[i0 + l], to = __shfl_sync(0xffffffffu, at, l) - 1;
-        const double d = page < v.pages ? page_score<T, D>(a, q, page, h, lane) : 0.0;
-        if (lane == 0) scores[to] = (float)d;
+      __syncthreads();
+      if (lane == 0) sh.warp[0][warp] = in, sh.warp[1][warp] = near;
+      __syncthreads();
+      if (!one && warp == 0) {
+        in = lane < kThreads / 32 ? sh.warp[0][lane] : 0u, near = lane < kThreads / 32 ? sh.warp[1][lane] : 0u;
+        in = __reduce_add_sync(0xffffffffu, in), near = __reduce_add_sync(0xffffffffu, near);
+        tell(group, sh.zones, make_uint2(in, near));
+      }
+      if (!one) sync(group);
+      in = near = 0;
+      if (one)
+        for (int w = 0; w < kThreads / 32; w++) in += sh.warp[0][w], near += sh.warp[1][w];
+      else
+        for (uint32_t c = 0; c < size; c++) in += sh.zones[c].x, near += sh.zones[c].y;
+      refine = (vague || tl == tl) && in + near != r.want;
+      if (refine && one && near <= kNear) {
+        // The near pages' f64 scores, and their order among one another.
+        refine = false, by_bit = true;
+        for (uint32_t i = t; i < (count + 31) / 32; i += kThreads) chosen[i] = 0;
+        for (uint32_t i = t; i < count; i += kThreads)
+          if (!forced(i) && zone(keys[i]) == 1) near_at[atomicAdd(&nears, 1u)] = i;
+        __syncthreads();
+        for (uint32_t i = warp; i < near; i += kThreads / 32) {
+          const double d = page_score<T, D>(a, q, table[near_at[i]], h, lane);
+          if (lane == 0) near_key[i] = order(d);
+        }
+        __syncthreads();
+        if (t < (int)near) {
+          uint32_t ahead_of = 0;
+          for (uint32_t i = 0; i < near; i++)
+            ahead_of += near_key[i] > near_key[t] || (near_key[i] == near_key[t] && near_at[i] < near_at[t]);
+          if (ahead_of < r.want - in) atomicOr(&chosen[near_at[t] / 32], 1u << (near_at[t] % 32));
+        }
+        __syncthreads();
       }
     }
+    if (!refine)
+      emit_taken(
+          group, sh, count, r.ties,
+          [&](uint32_t i) {
+            if (!by_bit) return state_of(r, keys[i], forced(from + i));
+            const int z = forced(i) ? 2 : zone(keys[i]);
+            return z == 1 ? (int)(chosen[i / 32] >> (i % 32) & 1) * 2 : z;
+          },
+          [&](uint32_t i, bool taken, uint32_t at) {
+            if (!taken) return;
+            out[at] = from + i;
+            if (scores) scores[at] = __uint_as_float(topk_bits(keys[i]));
+          });
   }
+  if (alone) {
+    if (rank == 0 && warp == 0 && t < (int)size)
+      *cluster.map_shared_rank(&sh.verdict, t) = make_float4(refine ? 1.f : 0.f, above, below, vague ? 1.f : 0.f);
+    cluster.sync();
+    refine = sh.verdict.x != 0.f, above = sh.verdict.y, below = sh.verdict.z, vague = sh.verdict.w != 0.f;
+  }
+  if (!refine) return;
+  // The near pages in f64, a CTA its own; the rest of the choice is made.
+  auto taken_first = [&](uint32_t i) { return forced(i) || zone(keys[i - first]) == 2; };
+  for (uint32_t i = warp; i < n; i += kThreads / 32) {
+    double d = 0.0;
+    const bool near = !forced(first + i) && zone(keys[i]) == 1;
+    if (near) d = page_score<T, D>(a, q, table[first + i], h, lane);
+    if (lane == 0) exact[i] = near ? order(d) : 0ull;
+  }
+  __syncthreads();
+  const Threshold<uint64_t> r64 = find(whole, sh, exact, n, first, take, taken_first);
+  emit_taken(
+      whole, sh, n, r64.ties, [&](uint32_t i) { return state_of(r64, exact[i], taken_first(first + i)); },
+      [&](uint32_t i, bool taken, uint32_t at) {
+        if (!taken) return;
+        out[at] = first + i;
+        if (scores) scores[at] = __uint_as_float(topk_bits(keys[i]));
+      });
 }
 
 // ------------------------------------------------------------ eviction
@@ -506,9 +728,10 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const EvictArgs a, uint3
   __syncthreads();
   cluster.barrier_wait();
   auto forced = [&](uint32_t i) { return i < a.sink || i + a.recent >= entries; };
-  const Threshold<uint32_t> r = find(cluster, sh, keys, n, first, min(a.budget, entries), forced);
+  const Group group{&cluster, size, rank};
+  const Threshold<uint32_t> r = find(group, sh, keys, n, first, min(a.budget, entries), forced);
   emit_taken(
-      cluster, sh, n, r.ties, [&](uint32_t i) { return state_of(r, keys[i], forced(first + i)); },
+      group, sh, n, r.ties, [&](uint32_t i) { return state_of(r, keys[i], forced(first + i)); },
       [&](uint32_t i, bool taken, uint32_t at) {
         if (taken) out[at] = first + i;
       });
@@ -575,15 +798,21 @@ __global__ void __launch_bounds__(256) move_kernel(const EvictArgs a) {
   }
 }
 
-// CTAs a cluster: as many as fill the GPU once, at least enough that the
-// slices fit shared memory; 0 when even the widest cluster's do not.
-uint32_t cluster_for(uint64_t items, uint64_t longest, size_t key_bytes, size_t room) {
+// CTAs a cluster: as many as fill the GPU once while each has `worth` keys, and
+// at least enough that the slices fit shared memory; 0 when even the widest
+// cluster's do not.
+uint32_t cluster_for(uint64_t items, uint64_t longest, uint32_t worth, size_t key_bytes, size_t room) {
   uint32_t c = 1;
-  while (c < kMaxCluster && ((longest + c - 1) / c * key_bytes > room || (items * c < 148 && longest / c > 256))) c *= 2;
+  while (c < kMaxCluster && ((longest + c - 1) / c * key_bytes > room || (items * c * 2 <= 148 && longest / c > worth))) c *= 2;
   return (longest + c - 1) / c * key_bytes > room ? 0 : c;
 }
 
 constexpr size_t kRoom = 196 * 1024;
+constexpr size_t kPagesRoom = 58 * 1024;   // beside the ring and q's operands (24 KiB at most)
+template <class T, int D>
+const void* select_of(bool many) {
+  return many ? (const void*)select_kernel<T, D, 8> : (const void*)select_kernel<T, D, 4>;
+}
 
 }  // namespace
 }  // namespace fz
@@ -605,26 +834,31 @@ extern "C" fz_status fz_paged_select(const fz_paged_kv* kv, const float* q, uint
     return paged_refuse(FZ_ERR_ARGUMENT, "a q stride shorter than its heads");
   if (top == 0 || (uint64_t)sink + recent > top) return paged_refuse(FZ_ERR_ARGUMENT, "top must be nonzero and at least sink + recent");
   const uint64_t items = (uint64_t)kv->sequences * kv->kv_heads;
-  const uint32_t c = cluster_for(items, kv->table_stride, 12, kRoom);
-  if (!c) return paged_refuse(FZ_ERR_NOT_SUPPORTED, "more pages a sequence than a cluster's shared memory holds scores of (133,000)");
+  const uint32_t c = cluster_for(items, kv->table_stride, 32, 13, kPagesRoom);
+  if (!c) return paged_refuse(FZ_ERR_NOT_SUPPORTED, "more pages a sequence than a cluster's shared memory holds scores of (36,000)");
   if (items * c > 0x7FFFFFFFull) return paged_refuse(FZ_ERR_ARGUMENT, "too many sequences");
   if (items == 0) return FZ_OK;
   const void* p[] = {kv->page_table, kv->lengths, kv->bounds, kv->error, q, blocks, scores};
   if ((st = paged_on_device(p, 7, "fz_paged_select"))) return st;
   a.q = q, a.q_stride = q_stride, a.group = heads / kv->kv_heads;
   a.top = top, a.sink = sink, a.recent = recent, a.blocks = blocks, a.scores = scores;
-  uint32_t slice = (kv->table_stride + c - 1) / c;
-  slice = (slice + 3) & ~3u;     // (q behind the keys is read 16 bytes at a time)
-  void* args[] = {&a, &slice};
-  const bool f16 = kv->type == FZ_KV_F16;
   const uint32_t d = kv->head_dim;
-  const void* fn = f16 ? (d == 64    ? (const void*)select_kernel<F16, 64>
-                          : d == 128 ? (const void*)select_kernel<F16, 128>
-                                     : (const void*)select_kernel<F16, 256>)
-                       : (d == 64    ? (const void*)select_kernel<Bf16, 64>
-                          : d == 128 ? (const void*)select_kernel<Bf16, 128>
-                                     : (const void*)select_kernel<Bf16, 256>);
-  return paged_launch(fn, dim3((uint32_t)(items * c)), dim3(kThreads), slice * 12 + a.group * d * 4, c, args, stream);
+  uint32_t slice = (kv->table_stride + c - 1) / c;
+  slice += slice & 1;
+  // The first CTA takes all scores where it has the room for them.
+  uint32_t together = (kv->table_stride + 31) / 32 * 32;
+  if (together * 4ull + slice * 8ull > kPagesRoom - 8192) together = 0;
+  void* args[] = {&a, &slice, &together};
+  const bool f16 = kv->type == FZ_KV_F16, many = a.group > 4;
+  const uint32_t tiles = f16 ? (many ? 2 : 1) : (many ? 3 : 2), all = together ? together : slice;
+  const void* fn = f16 ? (d == 64    ? select_of<F16, 64>(many)
+                          : d == 128 ? select_of<F16, 128>(many)
+                                     : select_of<F16, 256>(many))
+                       : (d == 64    ? select_of<Bf16, 64>(many)
+                          : d == 128 ? select_of<Bf16, 128>(many)
+                                     : select_of<Bf16, 256>(many));
+  return paged_launch(fn, dim3((uint32_t)(items * c)), dim3(kThreads),
+                      kRing + d / 8 * tiles * 256 + slice * 8 + all * 4 + (all + 31) / 32 * 4, c, args, stream);
 }
 
 extern "C" fz_status fz_paged_evict(const fz_paged_kv* from, const fz_paged_kv* to, uint32_t budget, uint32_t sink,
@@ -644,7 +878,7 @@ extern "C" fz_status fz_paged_evict(const fz_paged_kv* from, const fz_paged_kv* 
   if (std::min<uint64_t>(budget, longest) > room) return paged_refuse(FZ_ERR_ARGUMENT, "budget past the destination's table");
   const uint64_t items = (uint64_t)from->sequences * from->kv_heads;
   if (items > 65535) return paged_refuse(FZ_ERR_ARGUMENT, "more than 65,535 sequences times KV heads");
-  const uint32_t c = cluster_for(items, longest, 4, kRoom);
+  const uint32_t c = cluster_for(items, longest, 256, 4, kRoom);
   if (!c) return paged_refuse(FZ_ERR_NOT_SUPPORTED, "more entries a sequence than a cluster's shared memory holds weights of (401,000)");
   if (items == 0) return FZ_OK;
   const void* p[] = {from->keys, from->values, from->page_table, from->lengths, from->weights, from->error,

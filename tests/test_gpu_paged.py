@@ -216,8 +216,12 @@ def test_select(type, d, heads, kv, page, lengths, top, sink, recent):
             want = best(score, n, sink, recent, top)
             assert list(blocks[s, h, :len(want)]) == list(want)
             assert (blocks[s, h, len(want):] == NONE).all() and (scores[s, h, len(want):] == 0).all()
-            # one rounding to f32 of the 64-bit score
-            assert np.allclose(scores[s, h, :len(want)], score[want], rtol=2.0 ** -24, atol=0)
+            # f32 accuracy: 32 additions of a chain within 2^-23 of the products' sizes each, 16 of f32 sums, the
+            # parts of q to 2^-22 and to 2^-25 of its largest
+            G = heads // kv
+            x = q[s, h * G:(h + 1) * G].double().abs()
+            size = (x.sum(-1) + d / 8 * x.amax(-1)).max() * cache.bounds.double().abs().max()
+            assert np.abs(scores[s, h, :len(want)] - score[want]).max(initial=0) <= 88 * 2.0 ** -24 * float(size)
 
 
 def test_select_ties_go_to_the_lower_page_and_nan_comes_first():
@@ -247,6 +251,43 @@ def test_select_reads_near_ties_in_64_bits():
         b[:, 0], b[:, 1] = 32768.0, 2.0 ** -10 * i
     q[:, :, 0] = 1024.0
     assert list(u32(select(cache, q, 3)[0])[0, 0]) == [5, 6, 7]
+
+
+@pytest.mark.parametrize("pages,take", [(200, 50), (3000, 700), (13000, 1)])
+def test_select_many_near_ties(pages, take):
+    """Every page within f32's doubt of every other: a few, more than one CTA scores again, more than one CTA holds.
+    Scores 2^20 + k 2^-10, k many times the same: the largest k first, then the lower page."""
+    torch = torch_cuda()
+    cache = Cache([pages * 2], page=2, d=64, bounds=True)
+    k = np.random.default_rng(pages).integers(0, 40, pages)
+    rows = torch.from_numpy(cache.table_np[0].astype(np.int64)).cuda()
+    cache.bounds[rows] = torch.from_numpy(k / 1024.0).cuda().to(cache.dtype)[:, None, None, None]
+    cache.bounds[:, :, :, 0] = 1024.0
+    q = torch.zeros(1, 1, 64, device="cuda")
+    q[0, 0, 0], q[0, 0, 1] = 1024.0, 1.0
+    blocks, scores = select(cache, q, take)
+    want = best(1048576.0 + k / 1024.0, pages, 0, 0, take)
+    assert list(u32(blocks)[0, 0]) == list(want)
+    assert (scores - 1048576.0).abs().max() <= 1.0
+
+
+def test_select_infinite_queries_and_bounds():
+    """Scores of +-inf and NaN choose as their 64-bit values do."""
+    torch = torch_cuda()
+    cache = Cache([40 * 16], page=16, d=64, bounds=True)
+    bounds(cache)
+    q = randn(1, 2, 64)
+    for change in ("q", "bounds"):
+        if change == "q":
+            q[0, 0, 3] = float("inf")
+        else:
+            q[0, 0, 3] = 1.0
+            cache.bounds[int(cache.table_np[0, 7]), 0, 1, 3] = float("inf")
+            cache.bounds[int(cache.table_np[0, 9]), 0, :, 5] = -float("inf")
+        x, b = q[0].double()[:, None], cache.bounds[torch.from_numpy(cache.table_np[0].astype(np.int64)).cuda(), 0].double()
+        score = torch.where(x < 0, x * b[:, 0], x * b[:, 1]).sum(-1)
+        score = torch.where(torch.isnan(score).any(0), float("nan"), score.nan_to_num(-1e300, 1e308, -1e308).amax(0))
+        assert list(u32(select(cache, q, 9)[0])[0, 0]) == list(best(score.cpu().numpy(), 40, 0, 0, 9))
 
 
 def test_select_bad_page_is_reported_and_last():
