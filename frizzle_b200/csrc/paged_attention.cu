@@ -202,6 +202,8 @@ FZ_DEV bool next(const AttendArgs& a, Walk& w, uint32_t unit, uint32_t extra) {
   return false;
 }
 
+FZ_DEV void hint(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // The item a share begins with.
 FZ_DEV Walk begin(const Share& sh, uint32_t unit) {
   return Walk{sh.s, sh.h, (sh.l.count + unit - 1) / unit, sh.at, 0, sh.l};
@@ -269,6 +271,18 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   const uint32_t ring = smem_u32(smem) + warp * kSlots * kHalf;
   const PagedView& v = a.kv;
   const uint32_t G = a.group, KV = v.kv_heads;
+  // While the kernel before this one ends: what is read first, from HBM into L2
+  // (a hint, so it may still be written).
+  {
+    const uint64_t at = blockIdx.x * (uint64_t)kThreads + threadIdx.x, words = (uint64_t)v.sequences * v.table_stride;
+    if (at * 32 < v.sequences) hint(v.lengths + at * 32);
+    if (at * 32 < words) hint(v.table + at * 32);
+    if (at * 32 < (uint64_t)v.sequences * KV * a.top && a.blocks) hint(a.blocks + at * 32);
+    if (at < (uint64_t)v.sequences * KV * G * (D / 32)) {
+      const uint64_t row = KV * G * (D / 32);
+      hint(a.q + at / row * a.q_stride + at % row * 32);
+    }
+  }
   pdl_wait();
   pdl_launch_dependents();
 
@@ -402,6 +416,21 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   Where later = find();
   int slot = 0;                                    // of the next half to use
   int unit = warp;
+
+  // Sequences without entries: zeros, a warp a sequence (while the first copies come).
+  for (uint32_t s0 = (blockIdx.x * kWarps + warp) * 32; s0 < v.sequences; s0 += gridDim.x * kThreads) {
+    const uint32_t s = s0 + lane;
+    bool empty = false;
+    if (s < v.sequences) {
+      const List l = list_of(a, s);
+      if (__ldcg(v.lengths + s) > l.n) note(v, FZ_PAGED_BAD_LENGTH);
+      empty = l.count == 0;
+    }
+    for (uint32_t left = __ballot_sync(0xffffffffu, empty); left; left &= left - 1) {
+      float4* out = reinterpret_cast<float4*>(a.out + (s0 + __ffs(left) - 1) * a.out_stride);
+      for (uint32_t i = lane; i < KV * G * D / 4; i += 32) out[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
 
   while (some && mine(seg)) {
     const int from = max(seg.at, 0), to = min(seg.at + (int)seg.units, (int)units);
@@ -599,21 +628,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
     some = then;
   }
   copy_wait<0>();
-
-  // Sequences without entries: zeros, a warp a sequence.
-  for (uint32_t s0 = (blockIdx.x * kWarps + warp) * 32; s0 < v.sequences; s0 += gridDim.x * kThreads) {
-    const uint32_t s = s0 + lane;
-    bool empty = false;
-    if (s < v.sequences) {
-      const List l = list_of(a, s);
-      if (__ldcg(v.lengths + s) > l.n) note(v, FZ_PAGED_BAD_LENGTH);
-      empty = l.count == 0;
-    }
-    for (uint32_t left = __ballot_sync(0xffffffffu, empty); left; left &= left - 1) {
-      float4* out = reinterpret_cast<float4*>(a.out + (s0 + __ffs(left) - 1) * a.out_stride);
-      for (uint32_t i = lane; i < KV * G * D / 4; i += 32) out[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  }
 }
 
 // What is left once every CTA of attend_kernel is done, by two kinds of CTAs.
@@ -871,14 +885,17 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   a.scores = reinterpret_cast<float*>(w + at[5]);
   const uint64_t entries = (uint64_t)kv->table_stride * kv->page_slots;
   a.score_stride = (entries + kWeighed - 1) / kWeighed * kWeighed;
-  // The longest list an item can have, in tiles: with at most one a warp,
-  // items stay whole (no join, and no CTA needs every length).
   uint64_t most = entries;
   if (a.blocks) most = std::min<uint64_t>(most, (uint64_t)a.top * kv->page_slots);
   else if (a.window) most = std::min<uint64_t>(most, a.window);
   const uint32_t tile = 4096 / kv->head_dim;
   const uint64_t tiles = (most + tile - 1) / tile;
-  a.whole = tiles <= kWarps;
+  // Items stay whole, by their number alone (no CTA needs every length, and
+  // nothing is left to add up), where they have at most a tile a warp, or where
+  // even items of the longest list take no longer than cut ones (64 sequences of
+  // 2 KV heads and a window of 512: 14.4 us cut or left whole by their lengths, XX so).
+  const double cost = (double)tiles + kBegin, rounds = (double)((items + kCtas - 1) / kCtas);
+  a.whole = tiles <= kWarps || rounds * cost <= (double)items / kCtas * cost + 2 * kJoin;
   const uint32_t grid =
       (uint32_t)std::min<uint64_t>(kCtas, a.whole ? items : (items * tiles + kWarps - 1) / kWarps);
   void* args[] = {&a};
