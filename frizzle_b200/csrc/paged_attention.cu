@@ -62,27 +62,35 @@ FZ_DEV uint32_t listed(const AttendArgs& a, const uint32_t* blocks, uint32_t i, 
   return j < l.n && j >= l.first ? j : FZ_PAGED_NONE;
 }
 
-// The page and slot of entry i of (s, h)'s list; false where there is none to read.
-FZ_DEV bool place(const AttendArgs& a, uint32_t s, uint32_t h, uint32_t i, const List& l, uint32_t& page, uint32_t& slot) {
+// The table's word for entry i of (s, h)'s list and its slot in that page; slot
+// FZ_PAGED_NONE where there is no entry.
+FZ_DEV uint32_t look(const AttendArgs& a, uint32_t s, uint32_t h, uint32_t i, const List& l, uint32_t& slot) {
   const uint32_t* blocks = a.blocks ? a.blocks + ((size_t)s * a.kv.kv_heads + h) * a.top : nullptr;
   const uint32_t j = listed(a, blocks, i, l);
-  if (j == FZ_PAGED_NONE) return false;
-  page = a.kv.table[(size_t)s * a.kv.table_stride + j / a.kv.page_slots];
+  slot = FZ_PAGED_NONE;
+  if (j == FZ_PAGED_NONE) return FZ_PAGED_NONE;
   slot = j % a.kv.page_slots;
+  return a.kv.table[(size_t)s * a.kv.table_stride + j / a.kv.page_slots];
+}
+// Whether such a word and slot are an entry to read.
+FZ_DEV bool usable(const AttendArgs& a, uint32_t page, uint32_t slot) {
+  if (slot == FZ_PAGED_NONE) return false;
   if (page < a.kv.pages) return true;
   note(a.kv, FZ_PAGED_BAD_PAGE);
   return false;
 }
 
-constexpr uint32_t kBegin = kWarps;    // units that beginning an item costs
-constexpr uint32_t kJoin = kWarps;     // units that adding up shared items costs
+constexpr uint32_t kBegin = 3 * kWarps;   // units that beginning an item costs
+constexpr uint32_t kJoin = kWarps;        // units that adding up shared items costs
 
 // A CTA's share of all items' units (`unit` entries a unit), in order of
 // sequence and KV head: a contiguous run of ceil(all / CTAs) units, so that
 // every CTA reads as much as the others whatever the lengths.  Where a CTA has
 // several tiles a warp, `extra` units before each item stand for what beginning
-// it costs (measured at 8 x 32,768 entries of one KV head: CTAs with two items
-// ended 12 us after the others; counted as 8 units, 55 -> 40 us).  Where whole
+// it costs: the warps' barriers and the refilling of the copies' pipeline (8 x
+// 32,768 entries of one KV head: CTAs with two items ended 12 us after the
+// others, 55 us in all; counted as 8, 16 and 24 units 43, 42 and 40 us; 200
+// sequences of 500 entries 33, 30 and 29).  Where whole
 // items, the same number a CTA, take no longer than that and the joining (many
 // items of like length), items are not cut.  Called by the whole block.
 struct Share {
@@ -93,16 +101,19 @@ struct Share {
   List l;                  // its list
   uint64_t first, per;
 };
-FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit) {
-  __shared__ uint64_t sums[kWarps];
-  __shared__ uint2 counts[kWarps];
-  __shared__ Share found;
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const uint32_t S = a.kv.sequences, run = (S + kThreads - 1) / kThreads, s0 = min(S, t * run), s1 = min(S, s0 + run);
+// With up to 256 sequences every warp works it out for itself, a lane up to
+// eight sequences, without a barrier; beyond, the block together.
+template <bool BLOCK>
+FZ_DEV Share share_by(const AttendArgs& a, uint32_t unit, Share& found) {
+  constexpr uint32_t THREADS = BLOCK ? kThreads : 32;
+  const uint32_t t = BLOCK ? threadIdx.x : threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t S = a.kv.sequences, run = (S + THREADS - 1) / THREADS, s0 = min(S, t * run), s1 = min(S, s0 + run);
   const uint32_t ctas = gridDim.x, KV = a.kv.kv_heads;
   uint64_t tiles = 0;
   uint32_t some = 0, most = 0;
   List l{};
+#pragma unroll 8
   for (uint32_t s = s0; s < s1; s++) {
     l = list_of(a, s);
     const uint32_t u = (l.count + unit - 1) / unit;
@@ -119,20 +130,25 @@ FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit) {
     if (lane >= o) upto += x, some_upto += y;
   }
   most = __reduce_max_sync(0xffffffffu, most);
-  if (lane == 31) sums[warp] = upto, counts[warp] = make_uint2(some_upto, most);
+  uint64_t all = __shfl_sync(0xffffffffu, upto, 31), before = upto - tiles;
+  uint32_t any = __shfl_sync(0xffffffffu, some_upto, 31), some_before = some_upto - some;
   if (t == 0) found.units = found.items = 0;
-  __syncthreads();
-  uint64_t all = 0, before = 0;
-  uint32_t any = 0, some_before = 0;
+  if (BLOCK) {
+    __shared__ uint64_t sums[kWarps];
+    __shared__ uint2 counts[kWarps];
+    if (lane == 31) sums[warp] = upto, counts[warp] = make_uint2(some_upto, most);
+    __syncthreads();
+    all = 0, any = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; w++) {
-    if (w < warp) before += sums[w], some_before += counts[w].x;
-    all += sums[w];
-    any += counts[w].x;
-    most = max(most, counts[w].y);
+    for (int w = 0; w < kWarps; w++) {
+      if (w < warp) before += sums[w], some_before += counts[w].x;
+      all += sums[w];
+      any += counts[w].x;
+      most = max(most, counts[w].y);
+    }
+  } else {
+    __syncwarp();
   }
-  before += upto - tiles;
-  some_before += some_upto - some;
   const uint64_t items = (uint64_t)any * KV;
   const uint32_t extra = all * KV >= 2ull * kWarps * ctas ? kBegin : 0u;
   all = all * KV + items * extra;
@@ -164,8 +180,13 @@ FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit) {
     found.first = first;
     found.per = per;
   }
-  __syncthreads();
+  if (BLOCK) __syncthreads();
+  else __syncwarp();
   return found;
+}
+FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit) {
+  __shared__ Share found[kWarps];
+  return a.kv.sequences <= 256 ? share_by<false>(a, unit, found[threadIdx.x >> 5]) : share_by<true>(a, unit, found[0]);
 }
 
 // Walks a CTA's items that have entries: `at` is the item's first unit, counted
@@ -366,14 +387,20 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   // The copies' side: tile k of this warp is unit warp + 8 k of the CTA.
   Walk ahead = seg;
   bool more = some;
-  struct Where {
-    uint64_t off[(KT + 31) / 32];                  // this lane's rows, elements
-    uint64_t valid;                                // the tile's rows
+  constexpr int ROWS = (KT + 31) / 32;             // a lane's rows of a tile
+  struct Ask {
+    uint32_t page[ROWS], slot[ROWS], h;
     bool any;                                      // a tile
   };
+  struct Where {
+    uint64_t off[ROWS];                            // elements
+    uint64_t valid;                                // the tile's rows
+    bool any;
+  };
   int unit_ahead = warp;
-  auto find = [&]() {
-    Where w;
+  // The next tile's places: asked for before the products that hide the answer's way, made out after them.
+  auto ask = [&]() {
+    Ask w;
     w.any = more;
     while (w.any) {
       // (The units before an item's first hold nothing.)
@@ -382,17 +409,27 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
       if (!w.any || unit_ahead < ahead.at + (int)ahead.units) break;
       w.any = more = next(a, ahead, KT, extra);
     }
-    w.valid = 0;
+    w.h = ahead.h;
 #pragma unroll
-    for (int c = 0; c < (KT + 31) / 32; c++) {
-      uint32_t page = 0, slot = 0;
+    for (int c = 0; c < ROWS; c++) {
       const uint32_t row = lane + 32 * c;
-      const bool ok = w.any && row < KT &&
-                      place(a, ahead.s, ahead.h, (uint32_t)(unit_ahead - ahead.at) * KT + row, ahead.l, page, slot);
-      w.off[c] = ok ? element(v, page, slot, ahead.h) : 0;
-      w.valid |= (uint64_t)__ballot_sync(0xffffffffu, ok) << (32 * c);
+      w.page[c] = w.slot[c] = FZ_PAGED_NONE;
+      if (w.any && row < KT)
+        w.page[c] = look(a, ahead.s, ahead.h, (uint32_t)(unit_ahead - ahead.at) * KT + row, ahead.l, w.slot[c]);
     }
     unit_ahead += kWarps;
+    return w;
+  };
+  auto find = [&](const Ask& k) {
+    Where w;
+    w.any = k.any;
+    w.valid = 0;
+#pragma unroll
+    for (int c = 0; c < ROWS; c++) {
+      const bool ok = usable(a, k.page[c], k.slot[c]);
+      w.off[c] = ok ? element(v, k.page[c], k.slot[c], k.h) : 0;
+      w.valid |= (uint64_t)__ballot_sync(0xffffffffu, ok) << (32 * c);
+    }
     return w;
   };
   auto fetch = [&](const Where& w, const uint16_t* pool, int slot) {
@@ -408,12 +445,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
     }
     copy_commit();
   };
-  Where here = find(), soon = find();
+  const Ask ask0 = ask(), ask1 = ask();
+  Where here = find(ask0), soon = find(ask1);
   fetch(here, v.keys, 0);
   fetch(here, v.values, 1);
   fetch(soon, v.keys, 2);
   uint64_t valid = here.valid, valid_soon = soon.valid;
-  Where later = find();
   int slot = 0;                                    // of the next half to use
   int unit = warp;
 
@@ -485,6 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
       }
       __syncwarp();
       fetch(soon, v.values, slot);
+      const Ask asked = ask();
       slot = slot == kSlots - 1 ? 0 : slot + 1;
       float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
@@ -553,12 +591,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
         }
       }
       __syncwarp();
-      fetch(later, v.keys, slot);
+      soon = find(asked);
+      fetch(soon, v.keys, slot);
       slot = slot == kSlots - 1 ? 0 : slot + 1;
       valid = valid_soon;
-      valid_soon = later.valid;
-      soon = later;
-      later = find();
+      valid_soon = soon.valid;
     }
 
     // ---- the item's end: the warps' sums, maxima and outputs
@@ -738,8 +775,9 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, ui
     float* to[4];
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-      uint32_t page, slot;
-      const bool ok = place(a, s, kvh, i + c, l, page, slot);
+      uint32_t slot;
+      const uint32_t page = look(a, s, kvh, i + c, l, slot);
+      const bool ok = usable(a, page, slot);
       to[c] = ok ? v.weights + ((size_t)page * v.kv_heads + kvh) * v.page_slots + slot : nullptr;
     }
     if (!waited) {
@@ -893,8 +931,9 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   // Items stay whole, by their number alone (no CTA needs every length, and
   // nothing is left to add up), where they have at most a tile a warp, or where
   // even items of the longest list take no longer than cut ones (64 sequences of
-  // 2 KV heads and a window of 512: 14.4 us cut or left whole by their lengths, XX so).
-  const double cost = (double)tiles + kBegin, rounds = (double)((items + kCtas - 1) / kCtas);
+  // 2 KV heads and a window of 512: 14.4 us cut or left whole by their lengths, 11.0
+  // so).
+  const double cost = (double)tiles + kWarps, rounds = (double)((items + kCtas - 1) / kCtas);
   a.whole = tiles <= kWarps || rounds * cost <= (double)items / kCtas * cost + 2 * kJoin;
   const uint32_t grid =
       (uint32_t)std::min<uint64_t>(kCtas, a.whole ? items : (items * tiles + kWarps - 1) / kWarps);
