@@ -59,6 +59,9 @@ FZ_DEV uint64_t element(const PagedView& v, uint32_t page, uint32_t slot, uint32
   return page * v.page_stride + slot * v.slot_stride + head * v.head_stride;
 }
 
+// Into L2, before it is asked for (what it reads may still be written).
+FZ_DEV void hint(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // 16-byte copies into shared memory (zeros where not valid), by groups.
 FZ_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 FZ_DEV void copy16(uint32_t dst, const void* src, bool valid) {

@@ -280,27 +280,40 @@ FZ_DEV Threshold<uint32_t> find_alone(Shared& sh, const uint32_t* keys, uint32_t
   return r;
 }
 
-// emit(i, taken, rank) for every entry i of the CTA's n, the taken ones ranked in
-// ascending order over the cluster: state(i) 2 taken, 1 a tie, of which the cluster's first `ties`
-// are taken, 0 not.  Each thread takes a run of the slice.
+// emit(i, rank) for every taken entry i of the CTA's n, ranked in ascending order
+// over the cluster: state(i) 2 taken, 1 a tie, of which the cluster's first
+// `ties` are taken, 0 not.  Each warp takes a run of the slice, 32 at a time.
 template <class State, class Emit>
 FZ_DEV void emit_taken(const Group& group, Shared& sh, uint32_t n, uint32_t ties, State state, Emit emit) {
-  const uint32_t rank = group.rank, run = (n + kThreads - 1) / kThreads;
-  const uint32_t i0 = min(n, threadIdx.x * run), i1 = min(n, i0 + run);
-  __syncthreads();                       // (sh.warp is read)
-  uint2 mine = make_uint2(0, 0);
-  for (uint32_t i = i0; i < i1; i++) {
-    const int s = state(i);
-    mine.x += s == 2, mine.y += s == 1;
+  constexpr int W = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t run = (n + 32 * W - 1) / (32 * W) * 32, i0 = min(n, warp * run), i1 = min(n, i0 + run);
+  uint32_t more = 0, equal = 0;
+  for (uint32_t i = i0; i < i1; i += 32) {
+    const int s = i + lane < i1 ? state(i + lane) : 0;
+    more += __popc(__ballot_sync(0xffffffffu, s == 2)), equal += __popc(__ballot_sync(0xffffffffu, s == 1));
   }
-  uint2 at = block_scan(sh, mine);
-  if (threadIdx.x < 32) tell(group, sh.taken, make_uint2(sh.more, sh.equal));
-  sync(group);                        // (its arrival is the last thing a CTA does in another's shared memory)
-  for (uint32_t c = 0; c < rank; c++) at.x += sh.taken[c].x, at.y += sh.taken[c].y;
-  for (uint32_t i = i0; i < i1; i++) {
-    const int s = state(i);
-    emit(i, s == 2 || (s == 1 && at.y < ties), at.x + min(at.y, ties));
-    at.x += s == 2, at.y += s == 1;
+  __syncthreads();                       // (sh.warp is read)
+  if (lane == 0) sh.warp[0][warp] = more, sh.warp[1][warp] = equal;
+  __syncthreads();
+  more = equal = 0;
+  uint32_t all_more = 0, all_equal = 0;
+#pragma unroll
+  for (int w = 0; w < W; w++) {
+    if (w < warp) more += sh.warp[0][w], equal += sh.warp[1][w];
+    all_more += sh.warp[0][w], all_equal += sh.warp[1][w];
+  }
+  if (group.size > 1) {
+    if (warp == 0) tell(group, sh.taken, make_uint2(all_more, all_equal));
+    sync(group);                         // (its arrival is the last thing a CTA does in another's shared memory)
+    for (uint32_t c = 0; c < group.rank; c++) more += sh.taken[c].x, equal += sh.taken[c].y;
+  }
+  for (uint32_t i = i0; i < i1; i += 32) {
+    const int s = i + lane < i1 ? state(i + lane) : 0;
+    const uint32_t two = __ballot_sync(0xffffffffu, s == 2), one = __ballot_sync(0xffffffffu, s == 1), below = (1u << lane) - 1;
+    const uint32_t m = more + __popc(two & below), e = equal + __popc(one & below);
+    if (s == 2 || (s == 1 && e < ties)) emit(i + lane, m + min(e, ties));
+    more += __popc(two), equal += __popc(one);
   }
 }
 template <class K>
@@ -379,7 +392,7 @@ FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
 // The choice is wanted by the scores in 64 bits, and 64-bit conversions run at an
 // eighth of the rate of f32 arithmetic or less, so those are made for few pages
 // only.  First every page's score to f32 accuracy, off by at most
-//   E = (80 x 2^-24 + 2^-21) x (max_g sum |q| + D / 8 max |q|) x max |bound|
+//   E = 2^-24 x max_g (82 sum |q| + D / 2 max |q|) x max |bound|
 // (below), and the threshold T among those.  The take-th largest true score is
 // then within E of T: pages more than 2 E above T are in, pages more than 2 E
 // below are out, and only where more pages lie in between than are wanted are
@@ -395,9 +408,13 @@ FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
 // by cp.async three stages ahead, and no barrier or ldmatrix comes between.  Two
 // MMAs run into one f32 sum (32 additions to at least single precision, 2^-23 of
 // the products' sizes each), those are added by f32 (2 D / 32 of them, and the
-// parts): 64 + 16 times 2^-24, and 2^-22 and the subnormal parts' 2^-25 for what
-// q's parts leave out.  f32 lanes and shuffles instead took 60 us where this
-// takes 30 (16 sequences, 4 KV heads, up to 2,048 pages: 94 MB).
+// parts): 64 + 16 times 2^-24; what q's parts leave out is 2^-23 of a value, or
+// 2^-25 of the head's largest where a remainder is subnormal.
+//
+// Bound by HBM while it scores (4 D bytes a page), by barriers and single steps
+// while it chooses: 16 sequences of up to 2,048 pages and 4 KV heads, 94 MB, 34.6
+// us, 23 of them scoring the longest (all in f64: 90 us; f32 lanes and shuffles:
+// 61); one sequence of 2,032 pages 15.9 us (59, 25.7).
 //
 // Where one CTA's shared memory holds all the cluster's scores (`together`), the
 // first CTA gets them all and chooses alone, two cluster barriers in all; beyond
@@ -420,19 +437,40 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
   uint32_t* chosen = keys + (together ? together : slice);             // a bit a page: near the threshold and taken
   cg::cluster_group cluster = cg::this_cluster();
   cluster.barrier_arrive();                        // (waited for before the first word to another CTA)
+  const PagedView& v = a.kv;
+  // While the kernel before this one ends: what is read first, from HBM into L2.
+  if (t == 0) hint(v.lengths + blockIdx.x / cluster.num_blocks() / v.kv_heads);
+  for (uint32_t i = t * 32; i < slice; i += kThreads * 32)
+    hint(v.table + blockIdx.x / cluster.num_blocks() / v.kv_heads * (size_t)v.table_stride +
+         min(cluster.block_rank() * slice + i, v.table_stride - 1));
   pdl_wait();
   pdl_launch_dependents();
-  const PagedView& v = a.kv;
   const uint32_t size = cluster.num_blocks(), rank = cluster.block_rank(), G = a.group;
   const Group whole{&cluster, size, rank}, single{nullptr, 1, 0};
   const uint64_t item = blockIdx.x / size;
   const uint32_t s = (uint32_t)(item / v.kv_heads), h = (uint32_t)(item % v.kv_heads);
   const float* q = a.q + s * a.q_stride + (size_t)h * G * D;
-  const uint32_t entries = held(v, s);
-  if (t == 0 && rank == 0 && v.lengths[s] > entries) note(v, FZ_PAGED_BAD_LENGTH);
+  const uint32_t length = v.lengths[s];
+  // q: each head's size and scale (the largest to [1, 2)).
+  if (warp < GP) {
+    float sum = 0.f, top = 0.f;
+    for (int i = lane; i < D / 4 && warp < (int)G; i += 32) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(q + warp * D) + i);
+      sum += fabsf(x.x) + fabsf(x.y) + fabsf(x.z) + fabsf(x.w);
+      top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+    }
+    sum = warp_sum(sum), top = warp_max(top);
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);   // 2^(e - 127) <= top
+    if (lane == 0) norm[warp] = 82.f * sum + top * (D / 2), scale[warp] = top == INFINITY ? NAN : __uint_as_float((uint32_t)e << 23);
+  }
+  const uint32_t entries = min(length, v.table_stride * v.page_slots);
+  if (t == 0 && rank == 0 && length > entries) note(v, FZ_PAGED_BAD_LENGTH);
   const uint32_t pages = (entries + v.page_slots - 1) / v.page_slots;
   const uint32_t per = (pages + size - 1) / size, first = min(pages, rank * per), n = min(pages, first + per) - first;
   const uint32_t* table = v.table + (size_t)s * v.table_stride;
+  const bool alone = together && size > 1, one = alone || size == 1;   // one CTA chooses
+  for (uint32_t i = t; one && i < (pages + 31) / 32; i += kThreads) chosen[i] = 0;
+  if (t == 0) nears = 0;
 
   // The copies, kStages - 1 stages ahead of their use: rows g4 and g4 + 8 of the
   // tile, 16 bytes of every 64.
@@ -472,19 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
     out[i] = FZ_PAGED_NONE;
     if (scores) scores[i] = 0.f;
   }
-  // q: each head's size and scale (the largest to [1, 2)), then its parts.
-  if (warp < GP) {
-    float sum = 0.f, top = 0.f;
-    for (int i = lane; i < D / 4 && warp < (int)G; i += 32) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(q + warp * D) + i);
-      sum += fabsf(x.x) + fabsf(x.y) + fabsf(x.z) + fabsf(x.w);
-      top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
-    }
-    sum = warp_sum(sum), top = warp_max(top);
-    const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);   // 2^(e - 127) <= top
-    if (lane == 0) norm[warp] = sum + top * (D / 8), scale[warp] = top == INFINITY ? NAN : __uint_as_float((uint32_t)e << 23);
-  }
   __syncthreads();
+  // Its parts.
   {
     const uint32_t g = g4 % GP;
     const float down = __uint_as_float((254u << 23) - __float_as_uint(scale[g]));   // the reciprocal of a power of two
@@ -565,7 +592,6 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
   __syncthreads();
   cluster.barrier_wait();
   if (warp == 0) tell(whole, sh.bound, warp_max(lane < kThreads / 32 ? bound[lane] : 0.f));
-  const bool alone = together && size > 1;
   if (alone && rank) {
     uint32_t* all = cluster.map_shared_rank(keys, 0) + first;
     for (uint32_t i = t; i < n; i += kThreads) all[i] = keys[i];
@@ -575,7 +601,6 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
 
   // The threshold among them, by the first CTA alone or by all (their first
   // barrier makes the bounds seen).  A free page's zone: 2 in, 1 near T, 0 out.
-  const bool one = alone || size == 1;
   const uint32_t take = min(a.top, pages);
   auto forced = [&](uint32_t i) { return i < a.sink || i + a.recent >= pages; };
   bool refine = false;                             // too many near T for the first CTA: all of them score theirs in f64
@@ -595,15 +620,18 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
       float m = 0.f, norms = 0.f;
       for (uint32_t c = 0; c < size; c++) m = fmaxf(m, sh.bound[c]);
       for (uint32_t g = 0; g < G; g++) norms = norm[g] > norms || norm[g] != norm[g] ? norm[g] : norms;
-      const float e = 2.f * (80.f + 8.f) * 5.9604645e-8f * norms * m;
+      const float e = 2.f * 5.9604645e-8f * norms * m;
       // The ends' scores, as topk_key orders them.  (A NaN threshold: ties by the index, as in f64.)
       const float tl = __uint_as_float(topk_bits(r.prefix)), th = __uint_as_float(topk_bits(r.prefix | ~r.mask));
       below = tl - e, above = th == th ? th + e : INFINITY, vague = !(e < INFINITY);
       uint32_t in = 0, near = 0;
-      if (t == 0) nears = 0;
       for (uint32_t i = t; i < count; i += kThreads) {
         const int z = forced(from + i) ? 0 : zone(keys[i]);
         in += z == 2, near += z == 1;
+        if (z == 1 && one) {
+          const uint32_t at = atomicAdd(&nears, 1u);
+          if (at < kNear) near_at[at] = i;
+        }
       }
       in = __reduce_add_sync(0xffffffffu, in), near = __reduce_add_sync(0xffffffffu, near);
       __syncthreads();
@@ -624,10 +652,6 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
       if (refine && one && near <= kNear) {
         // The near pages' f64 scores, and their order among one another.
         refine = false, by_bit = true;
-        for (uint32_t i = t; i < (count + 31) / 32; i += kThreads) chosen[i] = 0;
-        for (uint32_t i = t; i < count; i += kThreads)
-          if (!forced(i) && zone(keys[i]) == 1) near_at[atomicAdd(&nears, 1u)] = i;
-        __syncthreads();
         for (uint32_t i = warp; i < near; i += kThreads / 32) {
           const double d = page_score<T, D>(a, q, table[near_at[i]], h, lane);
           if (lane == 0) near_key[i] = order(d);
@@ -650,8 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
             const int z = forced(i) ? 2 : zone(keys[i]);
             return z == 1 ? (int)(chosen[i / 32] >> (i % 32) & 1) * 2 : z;
           },
-          [&](uint32_t i, bool taken, uint32_t at) {
-            if (!taken) return;
+          [&](uint32_t i, uint32_t at) {
             out[at] = from + i;
             if (scores) scores[at] = __uint_as_float(topk_bits(keys[i]));
           });
@@ -675,8 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
   const Threshold<uint64_t> r64 = find(whole, sh, exact, n, first, take, taken_first);
   emit_taken(
       whole, sh, n, r64.ties, [&](uint32_t i) { return state_of(r64, exact[i], taken_first(first + i)); },
-      [&](uint32_t i, bool taken, uint32_t at) {
-        if (!taken) return;
+      [&](uint32_t i, uint32_t at) {
         out[at] = first + i;
         if (scores) scores[at] = __uint_as_float(topk_bits(keys[i]));
       });
@@ -690,6 +712,9 @@ struct EvictArgs {
   uint32_t* kept;
 };
 
+// The choice: 4 bytes an entry read, so bound by its barriers: 8 sequences of up
+// to 32,640 entries and 2 KV heads 18 us (49 while CTAs read one another's counts
+// instead of being told them), 1,500 entries 6 us.
 __global__ void __launch_bounds__(kThreads) keep_kernel(const EvictArgs a, uint32_t slice) {
   constexpr int BATCH = 8;                         // entries a thread asks for at once
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -739,14 +764,13 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const EvictArgs a, uint3
                                           : find(group, sh, keys, n, first, min(a.budget, entries), forced);
   emit_taken(
       group, sh, n, r.ties, [&](uint32_t i) { return state_of(r, keys[i], forced(first + i)); },
-      [&](uint32_t i, bool taken, uint32_t at) {
-        if (taken) out[at] = first + i;
-      });
+      [&](uint32_t i, uint32_t at) { out[at] = first + i; });
 }
 
 // The kept entries' keys and values, D / 8 lanes an entry, 16 bytes a lane, four
 // steps' loads at once; their weights; and the new length.  Memory bound: 4 x D
-// bytes read and written an entry.
+// bytes read and written an entry: 8 sequences, 2 KV heads, 4,080 entries, 134 MB,
+// 21 us (6.4 TB/s; 4 bytes a lane and a warp an entry: 45).
 template <int D>
 __global__ void __launch_bounds__(256) move_kernel(const EvictArgs a) {
   constexpr int LANES = D / 8, ROWS = 32 / LANES, STEPS = 4;

@@ -464,9 +464,11 @@ fz_status fz_attention_static(const float *q, const void *key_cache, const void 
  * KV head h of slot i of page p starts at keys (values) + p page_stride +
  * i slot_stride + h head_stride, in elements, head_dim elements in a row.  So
  * slot-major and head-major pages are both only strides.  Slots past a
- * sequence's length are never read, whatever they hold.  Pages that several
- * sequences share may be read by all of them; fz_paged_append, weight
- * accumulation and fz_paged_evict's `to` want pages of one sequence only.
+ * sequence's length are never read, whatever they hold.  An infinite key or value
+ * of an entry that takes part gives infinities or NaN.  Pages that several
+ * sequences share may be read by all of them (fz_paged_bounds too, where each
+ * holds them whole); fz_paged_append, weight accumulation and fz_paged_evict's
+ * `to` want pages of one sequence only.
  *
  * Lengths, tables and rows are device memory, so the host cannot check them:
  * the kernels do.  What they find out of range is skipped, never followed,

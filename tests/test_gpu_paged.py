@@ -82,12 +82,14 @@ def test_append(type, d, heads, kv, order, page):
     assert int(cache.error) == 0
 
 
-@pytest.mark.parametrize("rows_n,heads,kv,d", [(1, 4, 1, 256), (700, 4, 1, 256), (333, 16, 2, 64), (257, 5, 5, 128)])
+@pytest.mark.parametrize("rows_n,heads,kv,d", [(1, 4, 1, 256), (700, 4, 1, 256), (333, 16, 2, 64), (257, 5, 5, 128),
+                                               (2500, 4, 1, 256), (2100, 7, 3, 128), (2001, 13, 4, 64)])
 def test_append_many_rows(rows_n, heads, kv, d):
     cache = Cache([0], page=16, kv=kv, d=d, capacity=rows_n + 9)
     keys0, values0 = cache.keys.clone(), cache.values.clone()
-    order = np.random.default_rng(1).permutation(rows_n)             # rows in any order
-    rows = Rows(cache, heads, [0] * rows_n, order + 9, position=order * 3 + 100)
+    order = np.random.default_rng(1).permutation(rows_n)             # rows in any order, some of them padding
+    sequence = [NONE if i % 50 == 49 else 0 for i in range(rows_n)]
+    rows = Rows(cache, heads, sequence, order + 9, position=order * 3 + 100)
     rows.append(cache)
     check_append(cache, rows, keys0, values0, [0])
 
@@ -202,7 +204,7 @@ def test_bounds_nan_and_infinite_keys():
 @pytest.mark.parametrize("d,heads,kv,page,lengths,top,sink,recent", [
     (256, 4, 1, 16, [1000, 0, 1, 16, 700], 12, 1, 2), (128, 8, 2, 4, [2000, 1999], 100, 0, 0),
     (64, 15, 3, 8, [300, 50], 64, 3, 5), (256, 8, 1, 1, [5000], 257, 4, 4), (128, 2, 2, 16, [33, 90], 3, 1, 2),
-    (64, 1, 1, 2, [20000], 1, 0, 0)])
+    (64, 1, 1, 2, [20000], 1, 0, 0), (64, 5, 1, 1, [15000, 7], 300, 2, 2), (128, 16, 2, 1, [14000], 14000, 0, 9000)])
 def test_select(type, d, heads, kv, page, lengths, top, sink, recent):
     cache = Cache(lengths, page=page, kv=kv, d=d, type=type, bounds=True, seed=top)
     bounds(cache)
@@ -327,7 +329,8 @@ def test_attention_short(type, d, heads, kv, page, order, window):
 @pytest.mark.parametrize("lengths,heads,kv,d,page,window", [
     ([5000], 4, 1, 256, 16, 0), ([33000], 4, 1, 256, 32, 0), ([3000, 0, 2999, 1, 4097], 8, 1, 256, 16, 0),
     ([2500] * 40 + [3] * 40, 4, 2, 128, 24, 512), ([9000, 20], 16, 2, 64, 64, 0), ([700] * 149, 1, 1, 64, 16, 0),
-    ([1, 20000], 3, 1, 128, 13, 15000), ([4000] * 3, 12, 4, 256, 48, 0)])
+    ([1, 20000], 3, 1, 128, 13, 15000), ([4000] * 3, 12, 4, 256, 48, 0), ([600] * 70 + [0] * 10 + [5] * 20, 2, 1, 256, 16, 300),
+    ([0] * 100 + [300] * 90 + [0, 1] * 60 + [5000] + [0] * 40, 4, 2, 64, 16, 0), ([0] * 300, 2, 1, 128, 16, 0)])
 def test_attention_long(type, lengths, heads, kv, d, page, window):
     cache = Cache(lengths, page=page, kv=kv, d=d, type=type, seed=len(lengths)).hide()
     q = randn(len(lengths), heads, d, seed=1, scale=2.0)
@@ -341,7 +344,8 @@ def test_attention_long(type, lengths, heads, kv, d, page, window):
 @pytest.mark.parametrize("type", ["f16", "bf16"])
 @pytest.mark.parametrize("heads,kv,d,page,lengths,window,decay", [
     (4, 1, 256, 16, [40, 0, 1000, 5], 0, 1.0), (8, 1, 128, 24, [300, 129], 100, 0.5), (3, 3, 64, 8, [2000], 0, 0.0),
-    (10, 2, 256, 32, [5000, 1], 0, 1.0), (16, 2, 64, 16, [1000] * 30, 0, 1.0)])
+    (10, 2, 256, 32, [5000, 1], 0, 1.0), (16, 2, 64, 16, [1000] * 30, 0, 1.0), (4, 1, 256, 16, [600, 0, 5] * 40, 300, 0.25),
+    (5, 5, 128, 1, [90, 4000], 0, 1.0)])
 def test_attention_weights(type, heads, kv, d, page, lengths, window, decay):
     torch = torch_cuda()
     cache = Cache(lengths, page=page, kv=kv, d=d, type=type, weights=True, seed=9).hide()
@@ -504,7 +508,8 @@ def test_attention_far_offsets():
 @pytest.mark.parametrize("d,kv,page,to_page,order,lengths,budget,sink,recent", [
     (256, 1, 16, 16, "nhd", [1000, 0, 100, 64, 1], 64, 4, 10), (128, 3, 24, 7, "hnd", [500, 499], 200, 0, 0),
     (64, 2, 1, 16, "nhd", [40, 3], 1, 0, 0), (256, 1, 32, 32, "hnd", [9000], 4000, 16, 512),
-    (64, 4, 16, 64, "nhd", [70, 300, 20], 128, 64, 64), (128, 1, 16, 16, "nhd", [40], 100, 3, 3)])
+    (64, 4, 16, 64, "nhd", [70, 300, 20], 128, 64, 64), (128, 1, 16, 16, "nhd", [40], 100, 3, 3),
+    (64, 2, 16, 16, "nhd", [5000, 0, 40000, 3], 777, 0, 100)])
 def test_evict(type, d, kv, page, to_page, order, lengths, budget, sink, recent):
     torch = torch_cuda()
     a = Cache(lengths, page=page, kv=kv, d=d, type=type, order=order, weights=True, seed=budget).hide()
