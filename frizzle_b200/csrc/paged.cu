@@ -67,7 +67,8 @@ fz_status paged_view(const fz_paged_kv* kv, uint32_t need, PagedView* out) {
     return paged_refuse(FZ_ERR_ARGUMENT, "table, lengths, weights or error not 4-byte aligned");
   *out = PagedView{static_cast<uint16_t*>(kv->keys), static_cast<uint16_t*>(kv->values), kv->page_table, kv->lengths,
                    kv->weights, static_cast<uint16_t*>(kv->bounds), kv->error, kv->page_stride, kv->slot_stride,
-                   kv->head_stride, kv->sequences, kv->table_stride, kv->pages, kv->page_slots, kv->kv_heads};
+                   kv->head_stride, kv->sequences, kv->table_stride, kv->pages, kv->page_slots, kv->kv_heads,
+                   divisor(kv->page_slots)};
   return FZ_OK;
 }
 
@@ -150,8 +151,8 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs a, uint32_
   const uint32_t index = r.index[row];
   if (seq == FZ_PAGED_NONE) return;
   const bool in_table = seq < v.sequences && index < v.table_stride * v.page_slots;
-  const uint32_t page = in_table ? v.table[(size_t)seq * v.table_stride + index / v.page_slots] : 0u;
-  const uint32_t slot = index % v.page_slots;
+  const uint32_t page = in_table ? v.table[(size_t)seq * v.table_stride + index / v.slots] : 0u;
+  const uint32_t slot = in_table ? index % v.slots : 0u;
   float sn[4], cs[4];
   if (r.turns) {
     const double pos = (double)(r.position ? r.position[row] : index);
@@ -269,8 +270,10 @@ __global__ void __launch_bounds__(256, 3) bounds_kernel(const BoundsArgs a) {
       n = held(v, s);
       if (v.lengths[s] > n) note(v, FZ_PAGED_BAD_LENGTH);
       const uint32_t first = a.first ? a.first[s] : 0u;
-      page0 = first / v.page_slots;
-      if (first < n) count = (uint64_t)((n + v.page_slots - 1) / v.page_slots - page0) * v.kv_heads;
+      if (first < n) {
+        page0 = first / v.slots;
+        count = (uint64_t)((n + v.page_slots - 1) / v.slots - page0) * v.kv_heads;
+      }
     }
     uint64_t upto = count;
 #pragma unroll

@@ -9,6 +9,21 @@
 
 namespace fz {
 
+// Division of numbers below 2^31 by a divisor known beforehand (Granlund and
+// Montgomery 1994, theorem 4.2: multiplier floor(2^(31 + l) / d) + 1 with 2^l the
+// least power of two not below d): a product and a shift where a division by a
+// variable is some twenty instructions, at every look at a page table.
+struct Divisor {
+  uint32_t d, multiplier, shift;
+};
+inline Divisor divisor(uint32_t d) {
+  uint32_t l = 0;
+  while ((1ull << l) < d) l++;
+  return Divisor{d, (uint32_t)((1ull << (31 + l)) / d + 1), 31 + l};
+}
+FZ_DEV uint32_t operator/(uint32_t n, const Divisor& d) { return (uint32_t)(((uint64_t)n * d.multiplier) >> d.shift); }
+FZ_DEV uint32_t operator%(uint32_t n, const Divisor& d) { return n - n / d * d.d; }
+
 struct PagedView {
   uint16_t* keys;
   uint16_t* values;
@@ -19,6 +34,7 @@ struct PagedView {
   uint32_t* error;
   uint64_t page_stride, slot_stride, head_stride;
   uint32_t sequences, table_stride, pages, page_slots, kv_heads;
+  Divisor slots;                       // page_slots
 };
 
 // A cache element's type: f16 or bf16, its conversions to and from f32.

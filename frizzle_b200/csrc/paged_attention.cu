@@ -24,6 +24,7 @@ struct AttendArgs {
   uint32_t group, top, window;
   float scale_log2e, decay;
   uint32_t whole;          // items are never split
+  uint64_t recip;          // floor(2^64 / CTAs) + 1
   // Workspace.
   float* part_o;           // [kCtas][2][group][D] unnormalised outputs of a CTA's first and last item
   float2* part_ml;         // [kCtas][2][8] their maximum and sum
@@ -44,7 +45,7 @@ FZ_DEV List list_of(const AttendArgs& a, uint32_t s) {
   l.n = held(a.kv, s);
   l.first = a.window && l.n > a.window ? l.n - a.window : 0;
   const uint32_t slots = a.kv.page_slots;
-  l.count = a.blocks ? min(a.top, (l.n + slots - 1) / slots) * slots : l.n - l.first;
+  l.count = a.blocks ? min(a.top, (l.n + slots - 1) / a.kv.slots) * slots : l.n - l.first;
   return l;
 }
 
@@ -52,13 +53,13 @@ FZ_DEV List list_of(const AttendArgs& a, uint32_t s) {
 FZ_DEV uint32_t listed(const AttendArgs& a, const uint32_t* blocks, uint32_t i, const List& l) {
   if (i >= l.count) return FZ_PAGED_NONE;
   if (!blocks) return l.first + i;
-  const uint32_t slots = a.kv.page_slots, at = i / slots, b = blocks[at];
+  const uint32_t slots = a.kv.page_slots, at = i / a.kv.slots, b = blocks[at];
   if (b == FZ_PAGED_NONE) return FZ_PAGED_NONE;
-  if (b >= (l.n + slots - 1) / slots || (at && blocks[at - 1] >= b)) {
+  if (b >= (l.n + slots - 1) / a.kv.slots || (at && blocks[at - 1] >= b)) {
     note(a.kv, FZ_PAGED_BAD_BLOCK);
     return FZ_PAGED_NONE;
   }
-  const uint32_t j = b * slots + i % slots;
+  const uint32_t j = b * slots + (i - at * slots);
   return j < l.n && j >= l.first ? j : FZ_PAGED_NONE;
 }
 
@@ -69,8 +70,9 @@ FZ_DEV uint32_t look(const AttendArgs& a, uint32_t s, uint32_t h, uint32_t i, co
   const uint32_t j = listed(a, blocks, i, l);
   slot = FZ_PAGED_NONE;
   if (j == FZ_PAGED_NONE) return FZ_PAGED_NONE;
-  slot = j % a.kv.page_slots;
-  return a.kv.table[(size_t)s * a.kv.table_stride + j / a.kv.page_slots];
+  const uint32_t logical = j / a.kv.slots;
+  slot = j - logical * a.kv.page_slots;
+  return a.kv.table[(size_t)s * a.kv.table_stride + logical];
 }
 // Whether such a word and slot are an entry to read.
 FZ_DEV bool usable(const AttendArgs& a, uint32_t page, uint32_t slot) {
@@ -101,8 +103,8 @@ struct Share {
   List l;                  // its list
   uint64_t first, per;
 };
-// With up to 256 sequences every warp works it out for itself, a lane up to
-// eight sequences, without a barrier; beyond, the block together.
+// With up to 32 sequences every warp works it out for itself, without a barrier;
+// beyond, the block together.
 template <bool BLOCK>
 FZ_DEV Share share_by(const AttendArgs& a, uint32_t unit, Share& found) {
   constexpr uint32_t THREADS = BLOCK ? kThreads : 32;
@@ -113,7 +115,7 @@ FZ_DEV Share share_by(const AttendArgs& a, uint32_t unit, Share& found) {
   uint64_t tiles = 0;
   uint32_t some = 0, most = 0;
   List l{};
-#pragma unroll 8
+#pragma unroll 1
   for (uint32_t s = s0; s < s1; s++) {
     l = list_of(a, s);
     const uint32_t u = (l.count + unit - 1) / unit;
@@ -152,9 +154,10 @@ FZ_DEV Share share_by(const AttendArgs& a, uint32_t unit, Share& found) {
   const uint64_t items = (uint64_t)any * KV;
   const uint32_t extra = all * KV >= 2ull * kWarps * ctas ? kBegin : 0u;
   all = all * KV + items * extra;
-  const uint64_t even = (all >> 32) ? (all + ctas - 1) / ctas : ((uint32_t)all + (ctas - 1)) / ctas;
-  const uint64_t per = max((uint64_t)kWarps, even);
-  const uint64_t each = (items >> 32) ? (items + ctas - 1) / ctas : ((uint32_t)items + (ctas - 1)) / ctas;
+  // (Shares of a unit or an item more than needed do no harm, so a product with 2^64 / CTAs will do.)
+  const uint64_t even = ctas == 1 ? all : __umul64hi(all + ctas - 1, a.recip);
+  const uint64_t each = ctas == 1 ? items : __umul64hi(items + ctas - 1, a.recip);
+  const uint64_t per = even > kWarps ? even : kWarps;
   const bool whole = each * (most + extra) <= per + kJoin;
   // This thread's sequences, in units or in items.
   const uint64_t from = whole ? (uint64_t)some_before * KV : (before + (uint64_t)some_before * extra) * KV;
@@ -170,7 +173,11 @@ FZ_DEV Share share_by(const AttendArgs& a, uint32_t unit, Share& found) {
       base += (uint64_t)u * KV;
     }
     const uint64_t in = first - base;
-    found.h = KV == 1 ? 0u : (uint32_t)(in / u);
+    // (in / u: an estimate, put right.)
+    uint32_t h = KV == 1 ? 0u : min(KV - 1, (uint32_t)((float)in / (float)u));
+    while ((uint64_t)h * u > in) h--;
+    while ((uint64_t)(h + 1) * u <= in) h++;
+    found.h = h;
     found.at = whole ? 0 : (int)(extra + (int64_t)found.h * u - (int64_t)in);
     found.extra = extra;
     found.l = l;
@@ -186,7 +193,7 @@ FZ_DEV Share share_by(const AttendArgs& a, uint32_t unit, Share& found) {
 }
 FZ_DEV Share share_of(const AttendArgs& a, uint32_t unit) {
   __shared__ Share found[kWarps];
-  return a.kv.sequences <= 256 ? share_by<false>(a, unit, found[threadIdx.x >> 5]) : share_by<true>(a, unit, found[0]);
+  return a.kv.sequences <= 32 ? share_by<false>(a, unit, found[threadIdx.x >> 5]) : share_by<true>(a, unit, found[0]);
 }
 
 // Walks a CTA's items that have entries: `at` is the item's first unit, counted
@@ -320,8 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   bool some;
   if (a.whole) {
     const uint64_t all = (uint64_t)v.sequences * KV;
-    const uint32_t i0 = (uint32_t)(all * blockIdx.x / gridDim.x);
-    last_item = (uint32_t)(all * (blockIdx.x + 1) / gridDim.x);
+    const uint32_t each = (uint32_t)(all + gridDim.x - 1) / gridDim.x, i0 = (uint32_t)min(all, (uint64_t)blockIdx.x * each);
+    last_item = (uint32_t)min(all, (uint64_t)i0 + each);
     seg.s = i0 / KV, seg.h = i0 % KV;
     some = i0 < last_item;
     if (some) {
@@ -444,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         const int row = i * RPI + lane / CPR;
-        const uint64_t off = __shfl_sync(0xffffffffu, w.off[KT > 32 ? i / 8 : 0], row & 31);
+        const uint64_t off = __shfl_sync(0xffffffffu, ROWS == 1 || i < 8 ? w.off[0] : w.off[ROWS - 1], row & 31);
         copy16(base + row * (2 * D) + ((piece ^ (row & 7)) << 4), pool + off + piece * 8, (w.valid >> row) & 1);
       }
     }
@@ -661,8 +668,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
       __syncthreads();
     }
     if (seg.at >= 0 && threadIdx.x == 0) {
-      const uint64_t end = first + (uint64_t)(seg.at + (int64_t)seg.units) - 1;
-      const uint32_t ctas = is_whole ? 0u : (uint32_t)(end / per) - blockIdx.x + 1;
+      const uint32_t last = (uint32_t)seg.at + seg.units - 1;   // the item's last unit, from this CTA's first
+      const uint32_t ctas = is_whole ? 0u : last / (uint32_t)per + 1;
       if (!is_whole) a.heads[blockIdx.x] = make_uint4((uint32_t)item, ctas, from > 0 ? 1u : 0u, 0u);
       if (v.weights) a.origin[item] = make_uint4(blockIdx.x, ctas, from > 0 ? 1u : 0u, 0u);
     }
@@ -942,6 +949,7 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   a.whole = tiles <= kWarps || rounds * cost <= (double)items / kCtas * cost + 2 * kJoin;
   const uint32_t grid =
       (uint32_t)std::min<uint64_t>(kCtas, a.whole ? items : (items * tiles + kWarps - 1) / kWarps);
+  a.recip = grid > 1 ? ~0ull / grid + 1 : 0;
   void* args[] = {&a};
   const bool f16 = kv->type == FZ_KV_F16;
   const uint32_t d = kv->head_dim;

@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
   }
   const uint32_t entries = min(length, v.table_stride * v.page_slots);
   if (t == 0 && rank == 0 && length > entries) note(v, FZ_PAGED_BAD_LENGTH);
-  const uint32_t pages = (entries + v.page_slots - 1) / v.page_slots;
+  const uint32_t pages = (entries + v.page_slots - 1) / v.slots;
   const uint32_t per = (pages + size - 1) / size, first = min(pages, rank * per), n = min(pages, first + per) - first;
   const uint32_t* table = v.table + (size_t)s * v.table_stride;
   const bool alone = together && size > 1, one = alone || size == 1;   // one CTA chooses
@@ -741,8 +741,9 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const EvictArgs a, uint3
 #pragma unroll
     for (int c = 0; c < BATCH; c++) {
       const uint32_t i = i0 + c * kThreads, j = first + i;
-      page[c] = i < n ? table[j / v.page_slots] : FZ_PAGED_NONE;
-      slot[c] = j % v.page_slots;
+      const uint32_t logical = j / v.slots;
+      page[c] = i < n ? table[logical] : FZ_PAGED_NONE;
+      slot[c] = j - logical * v.page_slots;
     }
 #pragma unroll
     for (int c = 0; c < BATCH; c++)
@@ -795,15 +796,15 @@ __global__ void __launch_bounds__(256) move_kernel(const EvictArgs a) {
   uint64_t src = 0, dst = 0;
   bool ok = false;
   if (j != FZ_PAGED_NONE) {
-    const uint32_t from = f.table[(size_t)s * f.table_stride + j / f.page_slots],
-                   to = t.table[(size_t)s * t.table_stride + r / t.page_slots];
+    const uint32_t from = f.table[(size_t)s * f.table_stride + j / f.slots],
+                   to = t.table[(size_t)s * t.table_stride + r / t.slots];
     ok = from < f.pages && to < t.pages;
     if (to >= t.pages) note(t, FZ_PAGED_BAD_PAGE);
     if (ok) {
-      src = element(f, from, j % f.page_slots, h), dst = element(t, to, r % t.page_slots, h);
+      src = element(f, from, j % f.slots, h), dst = element(t, to, r % t.slots, h);
       if (t.weights)
-        t.weights[((size_t)to * t.kv_heads + h) * t.page_slots + r % t.page_slots] =
-            __ldcg(f.weights + ((size_t)from * f.kv_heads + h) * f.page_slots + j % f.page_slots);
+        t.weights[((size_t)to * t.kv_heads + h) * t.page_slots + r % t.slots] =
+            __ldcg(f.weights + ((size_t)from * f.kv_heads + h) * f.page_slots + j % f.slots);
     }
   }
   const uint32_t all = __ballot_sync(0xffffffffu, ok);
