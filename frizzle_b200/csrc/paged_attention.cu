@@ -278,9 +278,9 @@ FZ_DEV float fold(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - 
 //
 // Measured with it, d = 256, 4 heads, f16 (one CTA a sequence and KV head with
 // f32 products: 13.3 ms for the first): 8 sequences of up to 32,768 entries, 193
-// MB, 40 us (4.8 TB/s), 47 with their weights; up to 131,072 entries 125 us (6.2
-// TB/s); 2,048 selected entries of each 11.5 us; one of 36 entries 6.3 us, of
-// 4,096 10.2 us, some ten dependent reads, barriers and launches.
+// MB, 38 us (5.1 TB/s), 44 with their weights; up to 131,072 entries 125 us (6.2
+// TB/s); 2,048 selected entries of each 10.8 us; one of 36 entries 6.0 us, of
+// 4,096 9.4 us, some ten dependent reads, barriers and launches.
 template <class T, int D, int GP>
 __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a) {
   constexpr int KT = 4096 / D;                     // entries a tile
@@ -943,8 +943,8 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   // Items stay whole, by their number alone (no CTA needs every length, and
   // nothing is left to add up), where they have at most a tile a warp, or where
   // even items of the longest list take no longer than cut ones (64 sequences of
-  // 2 KV heads and a window of 512: 14.4 us cut or left whole by their lengths, 11.0
-  // so).
+  // 2 KV heads and a window of 512: 14.4 us cut or left whole by their lengths,
+  // 11.0 so).
   const double cost = (double)tiles + kWarps, rounds = (double)((items + kCtas - 1) / kCtas);
   a.whole = tiles <= kWarps || rounds * cost <= (double)items / kCtas * cost + 2 * kJoin;
   const uint32_t grid =
