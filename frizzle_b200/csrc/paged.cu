@@ -212,6 +212,8 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs a, uint32_
 
 // ------------------------------------------------------------ bounds
 
+constexpr uint32_t kWide = 128 * 256;        // a page's values of a head, from which a CTA takes it
+
 struct BoundsArgs {
   PagedView kv;
   const uint32_t* first;
@@ -242,25 +244,78 @@ FZ_DEV uint32_t most2<Bf16>(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// A page and KV head is D / 8 lanes, 16 bytes of each key a lane, the other
-// lanes of a warp (256 / D of them) every other slot; AHEAD slots' loads in
-// flight a lane.  A warp takes pages of the run first .. length - 1 of all
-// sequences in order, so the work is even whatever the lengths: the pages of
-// each 32 sequences are counted by one look at their lengths.  Memory bound:
-// every key is read once, 2 / page_slots of that written.  4 x 32,512 entries of
-// 2 x 256 (at 40 to 100 %), 93 MB: 15.6 us, 6.0 TB/s (a warp a page and 4-byte
-// loads: 24; 8 slots in flight and 4 CTAs an SM: 18.5); one page of 64 slots of
-// each of 16 sequences 4.2 us (14.8, 5.6).
+// The least and greatest of a page's slots, D / 8 lanes a key and 16 bytes a
+// lane, the other lanes of a warp (256 / D of them) every other slot, AHEAD
+// loads in flight a lane; a page by one warp, or (WIDE) by the CTA's eight, which
+// join in shared memory.
+template <class T, int D, bool WIDE>
+FZ_DEV void page_bounds(const PagedView& v, uint32_t page, uint32_t h, uint32_t slots, uint4 (*joined)[2][D / 8]) {
+  constexpr int LANES = D / 8, ROWS = 32 / LANES, AHEAD = WIDE ? 8 : 16, WARPS = WIDE ? 8 : 1;
+  const int lane = threadIdx.x & 31, part = lane % LANES, warp = threadIdx.x >> 5;
+  const uint16_t* k = v.keys + element(v, page, 0, h) + part * 8;
+  // (Slots past the page's held ones repeat its first.)
+  uint4 lo = *reinterpret_cast<const uint4*>(k), hi = lo;
+  for (uint32_t i = (WIDE ? warp * ROWS : 0) + lane / LANES; i < slots; i += ROWS * AHEAD * WARPS) {
+    uint4 x[AHEAD];
+#pragma unroll
+    for (int c = 0; c < AHEAD; c++) {
+      const uint32_t j = i + c * ROWS * WARPS;
+      x[c] = __ldcs(reinterpret_cast<const uint4*>(k + (j < slots ? j : 0u) * v.slot_stride));
+    }
+#pragma unroll
+    for (int c = 0; c < AHEAD; c++) {
+      lo = make_uint4(least2<T>(lo.x, x[c].x), least2<T>(lo.y, x[c].y), least2<T>(lo.z, x[c].z), least2<T>(lo.w, x[c].w));
+      hi = make_uint4(most2<T>(hi.x, x[c].x), most2<T>(hi.y, x[c].y), most2<T>(hi.z, x[c].z), most2<T>(hi.w, x[c].w));
+    }
+  }
+#pragma unroll
+  for (int o = LANES; o < 32; o <<= 1) {
+    const uint4 l = make_uint4(__shfl_xor_sync(0xffffffffu, lo.x, o), __shfl_xor_sync(0xffffffffu, lo.y, o),
+                               __shfl_xor_sync(0xffffffffu, lo.z, o), __shfl_xor_sync(0xffffffffu, lo.w, o));
+    const uint4 m = make_uint4(__shfl_xor_sync(0xffffffffu, hi.x, o), __shfl_xor_sync(0xffffffffu, hi.y, o),
+                               __shfl_xor_sync(0xffffffffu, hi.z, o), __shfl_xor_sync(0xffffffffu, hi.w, o));
+    lo = make_uint4(least2<T>(lo.x, l.x), least2<T>(lo.y, l.y), least2<T>(lo.z, l.z), least2<T>(lo.w, l.w));
+    hi = make_uint4(most2<T>(hi.x, m.x), most2<T>(hi.y, m.y), most2<T>(hi.z, m.z), most2<T>(hi.w, m.w));
+  }
+  uint4* b = reinterpret_cast<uint4*>(v.bounds + ((size_t)page * v.kv_heads + h) * 2 * D);
+  if (!WIDE) {
+    if (lane < LANES) b[part] = lo, b[LANES + part] = hi;
+    return;
+  }
+  if (lane < LANES) joined[warp][0][part] = lo, joined[warp][1][part] = hi;
+  __syncthreads();
+  if (threadIdx.x < 2 * LANES) {
+    const int side = threadIdx.x / LANES, at = threadIdx.x % LANES;
+    uint4 x = joined[0][side][at];
+#pragma unroll
+    for (int w = 1; w < 8; w++) {
+      const uint4 y = joined[w][side][at];
+      x = side ? make_uint4(most2<T>(x.x, y.x), most2<T>(x.y, y.y), most2<T>(x.z, y.z), most2<T>(x.w, y.w))
+               : make_uint4(least2<T>(x.x, y.x), least2<T>(x.y, y.y), least2<T>(x.z, y.z), least2<T>(x.w, y.w));
+    }
+    b[threadIdx.x] = x;
+  }
+  __syncthreads();
+}
+
+// The pages of first .. length - 1 of all sequences, counted 32 sequences at a
+// time by one look at their lengths and spread over the CTAs in order, so the
+// work is even whatever the lengths.  Memory bound: every key is read once, 2 /
+// page_slots of that written.  By CTAs where those have at most two pages (times
+// heads) each or pages are long (64 KiB of keys and more), else by warps: one
+// page of 64 slots of each of 16 sequences 2.9 us, by warps 4.2; 508 pages 5.8
+// and 8.0; 4 x 32,512 entries of 2 x 256 (at 40 to 100 %), 93 MB, in pages of 32
+// slots 15.7 us by warps (6.0 TB/s), by CTAs 26.4; of 128 slots 19.0 and 17.6, of
+// 512 42 and 15.8.  (4-byte loads: 24 us; 8 slots in flight and 4 CTAs an SM:
+// 18.5.)
 template <class T, int D>
 __global__ void __launch_bounds__(256, 3) bounds_kernel(const BoundsArgs a) {
-  constexpr int LANES = D / 8, ROWS = 32 / LANES, AHEAD = 16;
+  __shared__ uint4 joined[8][2][D / 8];
   pdl_wait();
   pdl_launch_dependents();
   const PagedView& v = a.kv;
-  const int lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES;
-  const uint64_t stride = (uint64_t)gridDim.x * 8;
-  uint64_t item = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);       // page and head, counted over all sequences
-  uint64_t before = 0;                                                 // of sequences s0 ..
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t turn = blockIdx.x;                                          // this CTA's place in the order, from where the last ones ended
   for (uint32_t s0 = 0; s0 < v.sequences; s0 += 32) {
     // Lane s: sequence s0 + s's entries, first touched page and number of pages times heads.
     const uint32_t s = s0 + lane;
@@ -282,50 +337,25 @@ __global__ void __launch_bounds__(256, 3) bounds_kernel(const BoundsArgs a) {
       if (lane >= o) upto += x;
     }
     const uint64_t all = __shfl_sync(0xffffffffu, upto, 31);
-    for (; item < before + all; item += stride) {
-      const uint64_t at = item - before;
+    const bool wide = all <= 2 * gridDim.x || (uint64_t)v.page_slots * D >= kWide;
+    const uint32_t step = wide ? gridDim.x : gridDim.x * 8;
+    for (uint64_t at = wide ? turn : turn * 8 + warp; at < all; at += step) {
       const int of = __popc(__ballot_sync(0xffffffffu, upto <= at));    // the sequence that holds it
       const uint64_t in = at - (__shfl_sync(0xffffffffu, upto, of) - __shfl_sync(0xffffffffu, count, of));
       const uint32_t entries = __shfl_sync(0xffffffffu, n, of);
       const uint32_t logical = __shfl_sync(0xffffffffu, page0, of) + (uint32_t)(in / v.kv_heads), h = (uint32_t)(in % v.kv_heads);
       const uint32_t page = v.table[(size_t)(s0 + of) * v.table_stride + logical];
+      const uint32_t slots = min(v.page_slots, entries - logical * v.page_slots);
       if (page >= v.pages) {
         if (lane == 0) note(v, FZ_PAGED_BAD_PAGE);
-        continue;
-      }
-      const uint32_t slots = min(v.page_slots, entries - logical * v.page_slots);
-      const uint16_t* k = v.keys + element(v, page, 0, h) + part * 8;
-      // (Slots past the page's held ones repeat its first.)
-      uint4 lo = *reinterpret_cast<const uint4*>(k), hi = lo;
-      for (uint32_t i = sub; i < slots; i += ROWS * AHEAD) {
-        uint4 x[AHEAD];
-#pragma unroll
-        for (int c = 0; c < AHEAD; c++) {
-          const uint32_t j = i + c * ROWS;
-          x[c] = __ldcs(reinterpret_cast<const uint4*>(k + (j < slots ? j : 0u) * v.slot_stride));
-        }
-#pragma unroll
-        for (int c = 0; c < AHEAD; c++) {
-          lo = make_uint4(least2<T>(lo.x, x[c].x), least2<T>(lo.y, x[c].y), least2<T>(lo.z, x[c].z), least2<T>(lo.w, x[c].w));
-          hi = make_uint4(most2<T>(hi.x, x[c].x), most2<T>(hi.y, x[c].y), most2<T>(hi.z, x[c].z), most2<T>(hi.w, x[c].w));
-        }
-      }
-#pragma unroll
-      for (int o = LANES; o < 32; o <<= 1) {
-        const uint4 l = make_uint4(__shfl_xor_sync(0xffffffffu, lo.x, o), __shfl_xor_sync(0xffffffffu, lo.y, o),
-                                   __shfl_xor_sync(0xffffffffu, lo.z, o), __shfl_xor_sync(0xffffffffu, lo.w, o));
-        const uint4 m = make_uint4(__shfl_xor_sync(0xffffffffu, hi.x, o), __shfl_xor_sync(0xffffffffu, hi.y, o),
-                                   __shfl_xor_sync(0xffffffffu, hi.z, o), __shfl_xor_sync(0xffffffffu, hi.w, o));
-        lo = make_uint4(least2<T>(lo.x, l.x), least2<T>(lo.y, l.y), least2<T>(lo.z, l.z), least2<T>(lo.w, l.w));
-        hi = make_uint4(most2<T>(hi.x, m.x), most2<T>(hi.y, m.y), most2<T>(hi.z, m.z), most2<T>(hi.w, m.w));
-      }
-      uint4* b = reinterpret_cast<uint4*>(v.bounds + ((size_t)page * v.kv_heads + h) * 2 * D);
-      if (sub == 0) {
-        b[part] = lo;
-        b[LANES + part] = hi;
+      } else if (wide) {
+        page_bounds<T, D, true>(v, page, h, slots, joined);
+      } else {
+        page_bounds<T, D, false>(v, page, h, slots, joined);
       }
     }
-    before += all;
+    const uint32_t used = (uint32_t)((wide ? all : (all + 7) / 8) % gridDim.x);
+    turn = turn >= used ? turn - used : turn + gridDim.x - used;
   }
 }
 
@@ -399,9 +429,8 @@ extern "C" fz_status fz_paged_bounds(const fz_paged_kv* kv, const uint32_t* firs
   const void* p[] = {kv->keys, kv->page_table, kv->lengths, kv->bounds, kv->error, first};
   if ((st = paged_on_device(p, 6, "fz_paged_bounds"))) return st;
   a.first = first;
-  // At most three CTAs an SM (each warp then takes several pages).
-  const uint64_t blocks = ((uint64_t)kv->table_stride * kv->kv_heads * kv->sequences + 7) / 8;
+  const uint64_t items = (uint64_t)kv->table_stride * kv->kv_heads * kv->sequences;
   void* args[] = {&a};
-  return paged_launch(pick<BoundsOf>(kv->type, kv->head_dim), dim3((uint32_t)std::min<uint64_t>(blocks, 3 * 148)), dim3(256), 0, 1,
+  return paged_launch(pick<BoundsOf>(kv->type, kv->head_dim), dim3((uint32_t)std::min<uint64_t>(items, 3 * 148)), dim3(256), 0, 1,
                       args, stream);
 }

@@ -165,7 +165,9 @@ def test_append_reports_bad_rows_and_pages_and_stores_the_rest():
 @pytest.mark.parametrize("type", ["f16", "bf16"])
 @pytest.mark.parametrize("d,kv,order,page,lengths,first", [
     (256, 1, "nhd", 16, [0, 1, 15, 16, 17, 100], None), (128, 3, "hnd", 24, [50, 47, 48, 0], [49, 47, 0, 0]),
-    (64, 2, "nhd", 1, [5, 3], [2, 3]), (256, 2, "hnd", 64, [300, 64], [128, 500])])
+    (64, 2, "nhd", 1, [5, 3], [2, 3]), (256, 2, "hnd", 64, [300, 64], [128, 500]),
+    (256, 1, "nhd", 150, [1000, 151], None), (64, 3, "hnd", 8, [3000] * 3 + [0] * 70 + [1, 700], None),
+    (128, 2, "nhd", 16, [100] * 200, [99] * 200), (64, 1, "nhd", 600, [599, 601, 5000], None)])
 def test_bounds(type, d, kv, order, page, lengths, first):
     torch = torch_cuda()
     cache = Cache(lengths, page=page, kv=kv, d=d, type=type, order=order, bounds=True).hide()
