@@ -687,9 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
 //
 // The others make the entries' weights from the scores and the items' maxima
 // and sums, 128 entries a warp at a time, four a lane, each entry written by the
-// one lane it falls to.  Where their entries lie they find out before
-// attend_kernel ends: neither it nor this kernel writes lengths, tables or
-// selected pages.
+// one lane it falls to.
 constexpr int kWeighed = 128;
 template <int D, bool F16>
 __global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, uint32_t ctas, uint32_t joins, uint32_t pieces) {
@@ -700,12 +698,12 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, ui
   __shared__ float reduce[2][kWarps];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const PagedView& v = a.kv;
+  pdl_wait();
+  pdl_launch_dependents();
   if (blockIdx.x < joins) {
     // The split items, in order.
     __shared__ uint4 split[kCtas];
     __shared__ uint32_t below[kWarps + 1];
-    pdl_wait();
-    pdl_launch_dependents();
     uint4 h = make_uint4(0, 0, 0, 0);
     if (t < (int)ctas) h = __ldcg(a.heads + t);
     const uint32_t any = __ballot_sync(0xffffffffu, h.y != 0);
@@ -773,7 +771,6 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, ui
     }
     return;
   }
-  bool waited = false;
   uint64_t of = ~0ull;                             // the item whose maxima and sums this warp holds
   float m = 0.f, inv = 0.f;                        // lanes 4 g ..: head g's
   const uint64_t units = (uint64_t)v.sequences * v.kv_heads * pieces;
@@ -791,11 +788,6 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, ui
       const uint32_t page = look(a, s, kvh, i + c, l, slot);
       const bool ok = usable(a, page, slot);
       to[c] = ok ? v.weights + ((size_t)page * v.kv_heads + kvh) * v.page_slots + slot : nullptr;
-    }
-    if (!waited) {
-      pdl_wait();
-      pdl_launch_dependents();
-      waited = true;
     }
     float4 x[8];
     float old[4] = {0.f, 0.f, 0.f, 0.f};
@@ -849,7 +841,6 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, ui
       if (to[c]) *to[c] = fmaf(a.decay, old[c], sum[c]);
     __syncwarp();
   }
-  if (!waited) pdl_wait();
 }
 
 template <class T, int D>

@@ -575,7 +575,8 @@ typedef struct fz_paged_query {
   uint32_t padding;
 } fz_paged_query;
 fz_status fz_paged_attention(const fz_paged_kv *kv, const fz_paged_query *query, void *stream);
-/* Bytes of workspace for the cache as described (its weights pointer counts) and `heads` query heads. */
+/* Bytes of workspace for the cache as described and `heads` query heads: a few MiB, with kv->weights 4 more a query
+ * head and table entry. */
 size_t fz_paged_attention_workspace(const fz_paged_kv *kv, uint32_t heads);
 
 /* Keeps at most `budget` entries of each sequence and KV head and writes them,

@@ -642,6 +642,81 @@ def test_decode_steps_captured_and_replayed(type, d, heads, kv):
     assert int(cache.error) == 0
 
 
+@pytest.mark.parametrize("window", [0, 37])
+def test_many_steps_without_a_pause(window):
+    """Forty steps queued at once (append, bounds, selection, attention of the selection with its weights, attention of
+    everything): each sees what the ones before it left, lengths, bounds, selections and weights among it."""
+    torch = torch_cuda()
+    lib = _native.load()
+    lengths, heads, kv, d, top, T = [150, 0, 33], 4, 1, 128, 5, 40
+    cache = Cache(lengths, page=8, kv=kv, d=d, capacity=200, weights=True, bounds=True, seed=5).hide()
+    cache.weights.zero_()
+    s = stream()
+    steps = []
+    for t in range(T):
+        rows = Rows(cache, heads, [0, 1, 2], [n + t for n in lengths], seed=100 + t)
+        q = rows.q_out.view(3, heads, d)
+        blocks, out, full = (torch.zeros(3, kv, top, dtype=torch.int32, device="cuda"), torch.empty_like(q), torch.empty_like(q))
+        steps.append((rows, q, blocks, out, full))
+    space = torch.empty(lib.fz_paged_attention_workspace(cache.desc, heads), dtype=torch.uint8, device="cuda")
+    plain = _native.PagedKv.from_buffer_copy(cache.desc)
+    plain.weights = None
+    bounds(cache)
+    torch.cuda.synchronize()
+    first = None
+    for rows, q, blocks, out, full in steps:
+        _native.check(lib.fz_paged_append(cache.desc, rows.desc, s))
+        _native.check(lib.fz_paged_bounds(cache.desc, first, s))
+        first = rows.dev[1].data_ptr()                   # (this step's entries: the page's other ones are in its bounds' page)
+        _native.check(lib.fz_paged_select(cache.desc, q.data_ptr(), heads * d, heads, top, 1, 1, blocks.data_ptr(), None, s))
+        attend(cache, q, 0.1, window, blocks=blocks, top=top, decay=1.0, workspace=space, out=out)
+        keep, cache.desc = cache.desc, plain
+        attend(cache, q, 0.1, window, workspace=space, out=full)
+        cache.desc = keep
+    torch.cuda.synchronize()
+    total = torch.zeros_like(cache.weights, dtype=torch.float64)
+    for t, (rows, q, blocks, out, full) in enumerate(steps):
+        cache.lengths = [n + t + 1 for n in lengths]
+        want, weights, bound = attend_exact(cache, q, 0.1, window, blocks)
+        check_out(out, want, bound)
+        check_out(full, *[attend_exact(cache, q, 0.1, window)[i] for i in (0, 2)])
+        for (i, h), (j, w) in weights.items():
+            p, o = cache.at(i, j)
+            total[p, h, o] += w
+        for i in range(3):
+            n = (cache.lengths[i] + 7) // 8
+            got = u32(blocks)[i, 0]
+            assert n - 1 in got[got != NONE] and 0 in got and len(set(got[got != NONE])) == min(top, n)
+    assert (cache.weights.double() - total).abs().max() < T * 1e-5
+    assert list(u32(cache.len)) == cache.lengths and int(cache.error) == 0
+
+
+def test_two_graphs_share_a_workspace():
+    """Graphs of two caches over one workspace, replayed in turn on one stream."""
+    torch = torch_cuda()
+    lib = _native.load()
+    caches = [Cache([2000, 3], page=16, d=256, weights=True, seed=1).hide(), Cache([700] * 5, page=32, d=256, weights=True, seed=2)]
+    qs = [randn(len(c.lengths), 4, 256, seed=i) for i, c in enumerate(caches)]
+    outs = [torch.zeros_like(q) for q in qs]
+    space = torch.empty(max(lib.fz_paged_attention_workspace(c.desc, 4) for c in caches), dtype=torch.uint8, device="cuda")
+    graphs = []
+    for c, q, out in zip(caches, qs, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            attend(c, q, 0.0625, decay=0.0, workspace=space, out=out)
+        graphs.append(graph)
+    for _ in range(10):
+        for graph in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    for c, q, out in zip(caches, qs, outs):
+        want, weights, bound = attend_exact(c, q, 0.0625)
+        check_out(out, want, bound)
+        for (s, h), (j, w) in weights.items():
+            p, o = c.at(s, j)
+            assert (c.weights[p, h, o].double() - w).abs().max() < 1e-5
+
+
 def test_two_streams_with_their_own_workspaces():
     torch = torch_cuda()
     caches = [Cache([3000, 10], page=16, d=256, seed=i).hide() for i in range(2)]
