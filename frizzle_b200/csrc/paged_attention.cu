@@ -92,9 +92,9 @@ constexpr uint32_t kJoin = kWarps;        // units that adding up shared items c
 // it costs: the warps' barriers and the refilling of the copies' pipeline (8 x
 // 32,768 entries of one KV head: CTAs with two items ended 12 us after the
 // others, 55 us in all; counted as 8, 16 and 24 units 43, 42 and 40 us; 200
-// sequences of 500 entries 33, 30 and 29).  Where whole
-// items, the same number a CTA, take no longer than that and the joining (many
-// items of like length), items are not cut.  Called by the whole block.
+// sequences of 500 entries 33, 30 and 29).  Where whole items, the same number a
+// CTA, take no longer than that and the joining (many items of like length),
+// items are not cut.  Called by the whole block.
 struct Share {
   uint32_t units, items;   // this CTA's; the one that does not count is large
   uint32_t extra;
@@ -248,6 +248,7 @@ FZ_DEV uint32_t transpose(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+
 // exp2 of a difference to the maximum of `m`'s side: 0 for a side without entries.
 FZ_DEV float fold(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
 
@@ -307,14 +308,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   // While the kernel before this one ends: what is read first, from HBM into L2
   // (a hint, so it may still be written).
   {
-    const uint64_t at = blockIdx.x * (uint64_t)kThreads + threadIdx.x, words = (uint64_t)v.sequences * v.table_stride;
+    const uint32_t at = blockIdx.x * kThreads + threadIdx.x, row = KV * G * (D / 32);   // (32 words a line)
     if (at * 32 < v.sequences) hint(v.lengths + at * 32);
-    if (at * 32 < words) hint(v.table + at * 32);
+    if (at * 32 < (uint64_t)v.sequences * v.table_stride) hint(v.table + at * 32);
     if (at * 32 < (uint64_t)v.sequences * KV * a.top && a.blocks) hint(a.blocks + at * 32);
-    if (at < (uint64_t)v.sequences * KV * G * (D / 32)) {
-      const uint64_t row = KV * G * (D / 32);
-      hint(a.q + at / row * a.q_stride + at % row * 32);
-    }
+    if (at < (uint64_t)v.sequences * row) hint(a.q + at / row * a.q_stride + at % row * 32);
   }
   pdl_wait();
   pdl_launch_dependents();
@@ -446,13 +444,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   };
   auto fetch = [&](const Where& w, const uint16_t* pool, int slot) {
     if (w.any) {
-      const uint32_t base = ring + slot * kHalf;
-      const int piece = lane % CPR;
+      // Row i RPI + sub, piece ^ (row & 7) of it (i RPI and sub have no bit in common).
+      const int piece = lane % CPR, sub = lane / CPR;
+      const uint32_t base = ring + slot * kHalf + sub * (2 * D), place = (piece ^ sub) << 4;
+      const uint16_t* from = pool + piece * 8;
+      const uint32_t low = (uint32_t)w.valid >> sub, high = (uint32_t)(w.valid >> 32) >> sub;
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        const int row = i * RPI + lane / CPR;
-        const uint64_t off = __shfl_sync(0xffffffffu, ROWS == 1 || i < 8 ? w.off[0] : w.off[ROWS - 1], row & 31);
-        copy16(base + row * (2 * D) + ((piece ^ (row & 7)) << 4), pool + off + piece * 8, (w.valid >> row) & 1);
+        const int row = i * RPI;
+        const uint64_t off = __shfl_sync(0xffffffffu, ROWS == 1 || i < 8 ? w.off[0] : w.off[ROWS - 1], (row & 31) + sub);
+        copy16(base + row * (2 * D) + (place ^ ((row & 7) << 4)), from + off, ((row < 32 ? low : high) >> (row & 31)) & 1);
       }
     }
     copy_commit();

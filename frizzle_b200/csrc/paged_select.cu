@@ -392,7 +392,7 @@ FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
 // The choice is wanted by the scores in 64 bits, and 64-bit conversions run at an
 // eighth of the rate of f32 arithmetic or less, so those are made for few pages
 // only.  First every page's score to f32 accuracy, off by at most
-//   E = 2^-24 x max_g (82 sum |q| + D / 2 max |q|) x max |bound|
+//   E = 2^-24 x max_g (88 sum |q| + D / 2 max |q|) x max |bound|
 // (below), and the threshold T among those.  The take-th largest true score is
 // then within E of T: pages more than 2 E above T are in, pages more than 2 E
 // below are out, and only where more pages lie in between than are wanted are
@@ -407,9 +407,9 @@ FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
 // bytes of a row as they lie for two steps' A operands; it copies them itself,
 // by cp.async three stages ahead, and no barrier or ldmatrix comes between.  Two
 // MMAs run into one f32 sum (32 additions to at least single precision, 2^-23 of
-// the products' sizes each), those are added by f32 (2 D / 32 of them, and the
-// parts): 64 + 16 times 2^-24; what q's parts leave out is 2^-23 of a value, or
-// 2^-25 of the head's largest where a remainder is subnormal.
+// the products' sizes each), those are added in f32 (2 D / 32 of them, and at
+// most four of parts): 64 + 20 times 2^-24; what q's parts leave out is 2^-23 of a
+// value, or 2^-25 of the head's largest where a remainder is subnormal.
 //
 // Bound by HBM while it scores (4 D bytes a page), by barriers and single steps
 // while it chooses: 16 sequences of up to 2,048 pages and 4 KV heads, 94 MB, 34.6
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
     }
     sum = warp_sum(sum), top = warp_max(top);
     const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);   // 2^(e - 127) <= top
-    if (lane == 0) norm[warp] = 82.f * sum + top * (D / 2), scale[warp] = top == INFINITY ? NAN : __uint_as_float((uint32_t)e << 23);
+    if (lane == 0) norm[warp] = 88.f * sum + top * (D / 2), scale[warp] = top == INFINITY ? NAN : __uint_as_float((uint32_t)e << 23);
   }
   const uint32_t entries = min(length, v.table_stride * v.page_slots);
   if (t == 0 && rank == 0 && length > entries) note(v, FZ_PAGED_BAD_LENGTH);

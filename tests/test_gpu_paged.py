@@ -220,8 +220,8 @@ def test_select(type, d, heads, kv, page, lengths, top, sink, recent):
             want = best(score, n, sink, recent, top)
             assert list(blocks[s, h, :len(want)]) == list(want)
             assert (blocks[s, h, len(want):] == NONE).all() and (scores[s, h, len(want):] == 0).all()
-            # f32 accuracy: 32 additions of a chain within 2^-23 of the products' sizes each, 16 of f32 sums, the
-            # parts of q to 2^-22 and to 2^-25 of its largest
+            # f32 accuracy: 32 additions of a chain within 2^-23 of the products' sizes each, 20 of f32 sums, the
+            # parts of q to 2^-23 and to 2^-25 of its largest
             G = heads // kv
             x = q[s, h * G:(h + 1) * G].double().abs()
             size = (x.sum(-1) + d / 8 * x.amax(-1)).max() * cache.bounds.double().abs().max()
@@ -273,6 +273,20 @@ def test_select_many_near_ties(pages, take):
     want = best(1048576.0 + k / 1024.0, pages, 0, 0, take)
     assert list(u32(blocks)[0, 0]) == list(want)
     assert (scores - 1048576.0).abs().max() <= 1.0
+
+
+@pytest.mark.parametrize("capacity", [12000, 36000])
+def test_select_largest_tables(capacity):
+    """The most shared memory a selection takes: 8 bf16 heads of 256 over the longest tables, chosen by one CTA or by all."""
+    cache = Cache([300, 7000], page=1, d=256, type="bf16", bounds=True, capacity=capacity, fill=0.0)
+    cache.keys.copy_(randn(*cache.keys.shape, seed=1))
+    bounds(cache)
+    q = randn(2, 8, 256, seed=2)
+    blocks = u32(select(cache, q, 500, 3, 3)[0])
+    for s, n in enumerate(cache.lengths):
+        want = best(page_scores(cache, q, s, 0), n, 3, 3, 500)
+        assert list(blocks[s, 0, :len(want)]) == list(want)
+    assert int(cache.error) == 0
 
 
 def test_select_infinite_queries_and_bounds():
@@ -535,6 +549,17 @@ def test_evict(type, d, kv, page, to_page, order, lengths, budget, sink, recent)
     assert list(u32(b.len)) == [min(n, budget) for n in lengths]
     assert (a.keys == keys0)[~torch.isnan(keys0)].all() and (a.weights == weights0).all()
     assert list(u32(a.len)) == lengths and int(a.error) == 0 and int(b.error) == 0
+
+
+def test_evict_longest_table():
+    """The most shared memory an eviction takes."""
+    a = Cache([70000, 10], page=16, d=64, weights=True, capacity=400000)
+    b = Cache([5000, 10], page=16, d=64, weights=True, seed=2)
+    kept = u32(evict(a, b, 5000, 1, 1))
+    want = best(a.weight(0, np.arange(70000), 0).cpu().numpy(), 70000, 1, 1, 5000)
+    assert list(kept[0, 0]) == list(want)
+    (p, o), (tp, to) = a.at(0, want), b.at(0, np.arange(5000))
+    assert (b.keys[tp, to, 0] == a.keys[p, o, 0]).all() and (b.weights[tp, 0, to] == a.weights[p, 0, o]).all()
 
 
 def test_evict_nan_weights_come_first_and_lengths_may_be_shared():
