@@ -43,7 +43,7 @@ struct Shared {
   uint2 taken[kMaxCluster];           // its keys above the threshold, and equal to it
   uint2 zones[kMaxCluster];           // its pages surely in, and near the threshold
   float bound[kMaxCluster];           // its greatest |bound|
-  float4 verdict;                     // the first CTA's choice: whether to refine, and the zones' ends
+  uint4 verdict;                      // the first CTA's word: whether to refine, and the range near the threshold
 };
 // The CTAs that choose together: a cluster, or one CTA alone.
 struct Group {
@@ -108,9 +108,9 @@ struct Threshold {
 // taken beforehand and count to `take`.  The digits, 9 bits each, begin at the
 // highest bit in which the keys differ, so that scores of like size take one
 // or two.
-template <class K, class Forced>
+template <class K, class Taken>
 FZ_DEV Threshold<K> find(const Group& group, Shared& sh, const K* keys, uint32_t n, uint32_t first, uint32_t take,
-                         Forced forced) {
+                         Taken forced) {
   const uint32_t size = group.size;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   Threshold<K> r{0, 0, 0, 0, false, false};
@@ -206,8 +206,8 @@ FZ_DEV Threshold<K> find(const Group& group, Shared& sh, const K* keys, uint32_t
 
 // The same by one CTA with all the keys: 8 bits a digit, their 256 bins summed by
 // one warp, so that a digit costs two barriers and little else.
-template <class Forced>
-FZ_DEV Threshold<uint32_t> find_alone(Shared& sh, const uint32_t* keys, uint32_t n, uint32_t take, Forced forced) {
+template <class Taken>
+FZ_DEV Threshold<uint32_t> find_alone(Shared& sh, const uint32_t* keys, uint32_t n, uint32_t take, Taken forced) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   Threshold<uint32_t> r{0, 0, 0, 0, false, false};
   uint32_t pinned = 0, least = ~0u, most = 0;
@@ -316,13 +316,22 @@ FZ_DEV void emit_taken(const Group& group, Shared& sh, uint32_t n, uint32_t ties
     more += __popc(two), equal += __popc(one);
   }
 }
+// Keys above a range 2, in it 1, below it 0; a threshold's range is the keys with its prefix.
 template <class K>
-FZ_DEV int state_of(const Threshold<K>& r, K key, bool forced) {
-  if (forced) return 2;
-  if (r.none) return 0;
-  const K k = key & r.mask;
-  return k > r.prefix ? 2 : k == r.prefix ? 1 : 0;
+struct Range {
+  K low, high;
+  FZ_DEV int side(K key) const { return key > high ? 2 : key >= low ? 1 : 0; }
+};
+template <class K>
+FZ_DEV Range<K> range_of(const Threshold<K>& r) {
+  return r.none ? Range<K>{~(K)0, ~(K)0} : Range<K>{r.prefix, r.prefix | ~r.mask};
 }
+// The entries taken beforehand: the first `sink` of n and the last `recent`.
+struct Forced {
+  uint32_t sink, tail;
+  FZ_DEV bool operator()(uint32_t i) const { return i < sink || i >= tail; }
+};
+FZ_DEV Forced forced_of(uint32_t n, uint32_t sink, uint32_t recent) { return Forced{sink, n > recent ? n - recent : 0u}; }
 
 // ------------------------------------------------------------ pages
 
@@ -412,9 +421,9 @@ FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
 // value, or 2^-25 of the head's largest where a remainder is subnormal.
 //
 // Bound by HBM while it scores (4 D bytes a page), by barriers and single steps
-// while it chooses: 16 sequences of up to 2,048 pages and 4 KV heads, 94 MB, 34.6
-// us, 23 of them scoring the longest (all in f64: 90 us; f32 lanes and shuffles:
-// 61); one sequence of 2,032 pages 15.9 us (59, 25.7).
+// while it chooses: 16 sequences of up to 2,048 pages and 4 KV heads, 94 MB, 33.2
+// us, 22 of them scoring the longest (all in f64: 90 us; f32 lanes and shuffles:
+// 61); one sequence of 2,032 pages 15.0 us (59, 25.7).
 //
 // Where one CTA's shared memory holds all the cluster's scores (`together`), the
 // first CTA gets them all and chooses alone, two cluster barriers in all; beyond
@@ -600,17 +609,12 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
   else __syncthreads();
 
   // The threshold among them, by the first CTA alone or by all (their first
-  // barrier makes the bounds seen).  A free page's zone: 2 in, 1 near T, 0 out.
+  // barrier makes the bounds seen).
   const uint32_t take = min(a.top, pages);
-  auto forced = [&](uint32_t i) { return i < a.sink || i + a.recent >= pages; };
+  const Forced forced = forced_of(pages, a.sink, a.recent);
   bool refine = false;                             // too many near T for the first CTA: all of them score theirs in f64
   Threshold<uint32_t> r{};
-  float above = 0.f, below = 0.f;
-  bool vague = false;                              // E is not finite: every page is near
-  auto zone = [&](uint32_t key) {
-    const float x = __uint_as_float(topk_bits(key));
-    return key == 0u ? 0 : vague ? 1 : x < below ? 0 : x > above || x != x ? 2 : 1;
-  };
+  Range<uint32_t> near_t{0, 0};                    // the keys near T
   if (!alone || rank == 0) {
     const Group group = one ? single : whole;
     const uint32_t from = one ? 0u : first, count = one ? pages : n;
@@ -618,15 +622,18 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
     bool by_bit = false;
     if (!r.every && !r.none) {
       float m = 0.f, norms = 0.f;
-      for (uint32_t c = 0; c < size; c++) m = fmaxf(m, sh.bound[c]);
-      for (uint32_t g = 0; g < G; g++) norms = norm[g] > norms || norm[g] != norm[g] ? norm[g] : norms;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; c++) m = c < (int)size ? fmaxf(m, sh.bound[c]) : m;
+#pragma unroll
+      for (int g = 0; g < GP; g++) norms = g < (int)G && (norm[g] > norms || norm[g] != norm[g]) ? norm[g] : norms;   // (NaN stays)
       const float e = 2.f * 5.9604645e-8f * norms * m;
       // The ends' scores, as topk_key orders them.  (A NaN threshold: ties by the index, as in f64.)
       const float tl = __uint_as_float(topk_bits(r.prefix)), th = __uint_as_float(topk_bits(r.prefix | ~r.mask));
-      below = tl - e, above = th == th ? th + e : INFINITY, vague = !(e < INFINITY);
+      const bool vague = !(e < INFINITY);          // every page is near (but those that are no pages, key 0)
+      near_t.low = vague ? 1u : max(1u, order(tl - e)), near_t.high = vague ? ~0u : order(th == th ? th + e : INFINITY);
       uint32_t in = 0, near = 0;
       for (uint32_t i = t; i < count; i += kThreads) {
-        const int z = forced(from + i) ? 0 : zone(keys[i]);
+        const int z = forced(from + i) ? 0 : near_t.side(keys[i]);
         in += z == 2, near += z == 1;
         if (z == 1 && one) {
           const uint32_t at = atomicAdd(&nears, 1u);
@@ -666,13 +673,13 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
         __syncthreads();
       }
     }
+    const Range<uint32_t> cut = by_bit ? near_t : range_of(r);
     if (!refine)
       emit_taken(
           group, sh, count, r.ties,
           [&](uint32_t i) {
-            if (!by_bit) return state_of(r, keys[i], forced(from + i));
-            const int z = forced(i) ? 2 : zone(keys[i]);
-            return z == 1 ? (int)(chosen[i / 32] >> (i % 32) & 1) * 2 : z;
+            const int z = forced(from + i) ? 2 : cut.side(keys[i]);
+            return z == 1 && by_bit ? (int)(chosen[i / 32] >> (i % 32) & 1) * 2 : z;
           },
           [&](uint32_t i, uint32_t at) {
             out[at] = from + i;
@@ -681,23 +688,24 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
   }
   if (alone) {
     if (rank == 0 && warp == 0 && t < (int)size)
-      *cluster.map_shared_rank(&sh.verdict, t) = make_float4(refine ? 1.f : 0.f, above, below, vague ? 1.f : 0.f);
+      *cluster.map_shared_rank(&sh.verdict, t) = make_uint4(refine, near_t.low, near_t.high, 0);
     cluster.sync();
-    refine = sh.verdict.x != 0.f, above = sh.verdict.y, below = sh.verdict.z, vague = sh.verdict.w != 0.f;
+    refine = sh.verdict.x != 0, near_t = Range<uint32_t>{sh.verdict.y, sh.verdict.z};
   }
   if (!refine) return;
   // The near pages in f64, a CTA its own; the rest of the choice is made.
-  auto taken_first = [&](uint32_t i) { return forced(i) || zone(keys[i - first]) == 2; };
+  auto taken_first = [&](uint32_t i) { return forced(i) || near_t.side(keys[i - first]) == 2; };
   for (uint32_t i = warp; i < n; i += kThreads / 32) {
     double d = 0.0;
-    const bool near = !forced(first + i) && zone(keys[i]) == 1;
+    const bool near = !forced(first + i) && near_t.side(keys[i]) == 1;
     if (near) d = page_score<T, D>(a, q, table[first + i], h, lane);
     if (lane == 0) exact[i] = near ? order(d) : 0ull;
   }
   __syncthreads();
   const Threshold<uint64_t> r64 = find(whole, sh, exact, n, first, take, taken_first);
+  const Range<uint64_t> cut = range_of(r64);
   emit_taken(
-      whole, sh, n, r64.ties, [&](uint32_t i) { return state_of(r64, exact[i], taken_first(first + i)); },
+      whole, sh, n, r64.ties, [&](uint32_t i) { return taken_first(first + i) ? 2 : cut.side(exact[i]); },
       [&](uint32_t i, uint32_t at) {
         out[at] = first + i;
         if (scores) scores[at] = __uint_as_float(topk_bits(keys[i]));
@@ -759,12 +767,13 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const EvictArgs a, uint3
   }
   __syncthreads();
   cluster.barrier_wait();
-  auto forced = [&](uint32_t i) { return i < a.sink || i + a.recent >= entries; };
+  const Forced forced = forced_of(entries, a.sink, a.recent);
   const Group group = size == 1 ? Group{nullptr, 1, 0} : Group{&cluster, size, rank};
   const Threshold<uint32_t> r = size == 1 ? find_alone(sh, keys, n, min(a.budget, entries), forced)
                                           : find(group, sh, keys, n, first, min(a.budget, entries), forced);
+  const Range<uint32_t> cut = range_of(r);
   emit_taken(
-      group, sh, n, r.ties, [&](uint32_t i) { return state_of(r, keys[i], forced(first + i)); },
+      group, sh, n, r.ties, [&](uint32_t i) { return forced(first + i) ? 2 : cut.side(keys[i]); },
       [&](uint32_t i, uint32_t at) { out[at] = first + i; });
 }
 

@@ -308,6 +308,16 @@ def test_select_infinite_queries_and_bounds():
         assert list(u32(select(cache, q, 9)[0])[0, 0]) == list(best(score.cpu().numpy(), 40, 0, 0, 9))
 
 
+@pytest.mark.parametrize("heads", [2, 8])
+def test_select_a_query_head_of_nan(heads):
+    """Every page scores NaN by the first head, whatever the others: the lowest pages, after what is forced."""
+    cache = Cache([40 * 16], page=16, d=64, bounds=True)
+    bounds(cache)
+    q = randn(1, heads, 64)
+    q[0, 0, 3] = float("nan")
+    assert list(u32(select(cache, q, 9, 0, 2)[0])[0, 0]) == [0, 1, 2, 3, 4, 5, 6, 38, 39]
+
+
 def test_select_bad_page_is_reported_and_last():
     cache = Cache([10 * 16], page=16, d=64, bounds=True)
     bounds(cache)
