@@ -655,7 +655,8 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
         for (int w = 0; w < kThreads / 32; w++) in += sh.warp[0][w], near += sh.warp[1][w];
       else
         for (uint32_t c = 0; c < size; c++) in += sh.zones[c].x, near += sh.zones[c].y;
-      refine = (vague || tl == tl) && in + near != r.want;
+      // (Fewer: the threshold is among what are no pages, and ties there go by the index.)
+      refine = (vague || tl == tl) && in + near > r.want;
       if (refine && one && near <= kNear) {
         // The near pages' f64 scores, and their order among one another.
         refine = false, by_bit = true;

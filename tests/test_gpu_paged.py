@@ -318,6 +318,23 @@ def test_select_a_query_head_of_nan(heads):
     assert list(u32(select(cache, q, 9, 0, 2)[0])[0, 0]) == [0, 1, 2, 3, 4, 5, 6, 38, 39]
 
 
+@pytest.mark.parametrize("take", [7, 8, 9, 10])
+def test_select_bad_pages_with_an_infinite_bound(take):
+    """Pages that are none come last in every case, and every word is written."""
+    cache = Cache([11 * 16], page=16, d=64, bounds=True)
+    bounds(cache)
+    bad = cache.table.clone()
+    bad[0, 4] = bad[0, 6] = bad[0, 9] = -1
+    cache.desc.page_table = bad.data_ptr()
+    cache.bounds[int(cache.table_np[0, 7]), 0, 1, 3] = float("inf")
+    q = randn(1, 1, 64).abs()
+    score = page_scores(cache, q, 0, 0)
+    score[[4, 6, 9]] = -float("inf")
+    blocks, _ = select(cache, q, take)
+    assert list(u32(blocks)[0, 0]) == list(best(score, 11, 0, 0, take))
+    assert int(cache.error) == 1
+
+
 def test_select_bad_page_is_reported_and_last():
     cache = Cache([10 * 16], page=16, d=64, bounds=True)
     bounds(cache)
