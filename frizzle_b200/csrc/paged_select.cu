@@ -406,8 +406,8 @@ FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
 // then within E of T: pages more than 2 E above T are in, pages more than 2 E
 // below are out, and only where more pages lie in between than are wanted are
 // those scored in f64 and chosen among by that (a page or two of two thousand,
-// as a rule).  With a score or a bound that is not finite, E is not either, and
-// every page is.
+// as a rule).  Where that product of sizes is not finite (an infinite bound, a
+// NaN query, scores about the largest f32), every page is.
 //
 // The scores are products of the pages' rows of 2 D least and greatest keys with
 // q's negative and positive parts: mma.sync m16n8k16 with 16 pages in M and the
@@ -419,6 +419,13 @@ FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
 // the products' sizes each), those are added in f32 (2 D / 32 of them, and at
 // most four of parts): 64 + 20 times 2^-24; what q's parts leave out is 2^-23 of a
 // value, or 2^-25 of the head's largest where a remainder is subnormal.
+//
+// q is scaled by powers of two, its largest value to [1, 2) for f16, to 2^-12 of
+// that for bf16, whose bounds may be as large as an f32: no sum of 2 D products
+// overflows then (2^9 x 2^-11 x the largest).  At the other end a product may be
+// lost below the least normal f32: 2 D x 3 of them are at most 2^-24 of a head's
+// size with bounds of 10^-26, so E takes no smaller bound; a score itself is
+// rounded at 2^-149, twice, and 2^12 times that: less than 10^-40, which E adds.
 //
 // Bound by HBM while it scores (4 D bytes a page), by barriers and single steps
 // while it chooses: 16 sequences of up to 2,048 pages and 4 KV heads, 94 MB, 33.2
@@ -432,6 +439,7 @@ template <class T, int D, int GP>
 __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a, uint32_t slice, uint32_t together) {
   constexpr int STEPS = D / 8, NT = (Parts<T>::N * GP + 7) / 8;        // 16-product steps a page; column tiles
   constexpr uint32_t STAGES = D / 32;                                  // stages (4 steps) a tile of 16 pages
+  constexpr float kUp = T::kType == FZ_KV_F16 ? 1.f : 4096.f, kDown = 1.f / kUp;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Shared sh;
   __shared__ float norm[8], scale[8], bound[kThreads / 32];
@@ -531,7 +539,8 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
       const bool least = at < D;
       const float y[4] = {(x.x < 0.f) == least ? x.x : x.x * 0.f, (x.y < 0.f) == least ? x.y : x.y * 0.f,
                           (x.z < 0.f) == least ? x.z : x.z * 0.f, (x.w < 0.f) == least ? x.w : x.w * 0.f};
-      const Parts<T> p0 = parts<T>(y[0] * down, y[1] * down), p1 = parts<T>(y[2] * down, y[3] * down);
+      const Parts<T> p0 = parts<T>(y[0] * down * kDown, y[1] * down * kDown),
+                     p1 = parts<T>(y[2] * down * kDown, y[3] * down * kDown);
 #pragma unroll
       for (int c = 0; c < NT; c++)
         qf[(k * NT + c) * 32 + lane] = GP == 8 ? make_uint2(p0.w[c], p1.w[c])
@@ -584,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
 #pragma unroll
       for (int c = 1; c < NT; c++) x += sum[c][2 * r], y += sum[c][2 * r + 1];
       if (GP == 4) x += __shfl_xor_sync(0xffffffffu, x, 2), y += __shfl_xor_sync(0xffffffffu, y, 2);
-      best[r] = max(has0 ? order(x * c0) : 0u, has1 ? order(y * c1) : 0u);
+      best[r] = max(has0 ? order(x * c0 * kUp) : 0u, has1 ? order(y * c1 * kUp) : 0u);
       best[r] = max(best[r], __shfl_xor_sync(0xffffffffu, best[r], 1));
       if (GP == 8) best[r] = max(best[r], __shfl_xor_sync(0xffffffffu, best[r], 2));
       const uint32_t i = tile * 16 + g4 + 8 * r, page = __shfl_sync(0xffffffffu, mine, g4 + 8 * r);
@@ -626,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
       for (int c = 0; c < kMaxCluster; c++) m = c < (int)size ? fmaxf(m, sh.bound[c]) : m;
 #pragma unroll
       for (int g = 0; g < GP; g++) norms = g < (int)G && (norm[g] > norms || norm[g] != norm[g]) ? norm[g] : norms;   // (NaN stays)
-      const float e = 2.f * 5.9604645e-8f * norms * m;
+      const float e = 2.f * 5.9604645e-8f * (norms * fmaxf(m, 1e-26f)) + 1e-40f;
       // The ends' scores, as topk_key orders them.  (A NaN threshold: ties by the index, as in f64.)
       const float tl = __uint_as_float(topk_bits(r.prefix)), th = __uint_as_float(topk_bits(r.prefix | ~r.mask));
       const bool vague = !(e < INFINITY);          // every page is near (but those that are no pages, key 0)

@@ -289,6 +289,21 @@ def test_select_largest_tables(capacity):
     assert int(cache.error) == 0
 
 
+@pytest.mark.parametrize("type,q_scale,bound", [
+    ("bf16", 1e-5, 3e38), ("bf16", 1e-36, 3e38), ("bf16", 1.0, 3e38), ("bf16", 1e37, 1e-38), ("bf16", 1.0, 1e-38),
+    ("bf16", 1e-6, 1e-38), ("bf16", 1e-41, 1.0), ("f16", 1e-41, 1.0), ("f16", 1e34, 6e4), ("f16", 1e34, 1e-6),
+    ("f16", 1e-36, 1e-6)])
+def test_select_at_the_ends_of_f32(type, q_scale, bound):
+    """Sums that pass the largest f32 by the way, products and scores below the least normal one."""
+    torch = torch_cuda()
+    cache = Cache([600 * 16], page=16, d=256, type=type, bounds=True)
+    b = torch.rand(cache.bounds.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) * 2 - 1
+    cache.bounds.copy_(torch.sort(b, dim=2).values * bound)          # least keys below the greatest
+    q = torch.clamp(randn(1, 3, 256, seed=6), -3, 3) * q_scale
+    blocks, _ = select(cache, q, 60)
+    assert list(u32(blocks)[0, 0]) == list(best(page_scores(cache, q, 0, 0), 600, 0, 0, 60))
+
+
 def test_select_infinite_queries_and_bounds():
     """Scores of +-inf and NaN choose as their 64-bit values do."""
     torch = torch_cuda()
