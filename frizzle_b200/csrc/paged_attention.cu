@@ -376,8 +376,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
     float top = largest[g * PER];
 #pragma unroll
     for (int i = 1; i < PER; i++) top = fmaxf(top, largest[g * PER + i]);
-    const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);   // 2^(e - 127) <= top, normal and inverse normal
-    const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
+    uint32_t e = query_exponent<T>(top);
+    // (With a scale about the largest f32 the room for keys of that size is given up: the factor stays finite.)
+    if (T::kType != FZ_KV_F16 && !(__uint_as_float(e << 23) * a.scale_log2e < INFINITY)) e -= 10;
+    const float down = __uint_as_float((254 - e) << 23), up = __uint_as_float(e << 23);
     const float2* q = reinterpret_cast<const float2*>(raw) + g * (D / 2) + t4;
     for (int k = warp; k < KS; k += kWarps) {
       const float2 x = q[8 * k], y = q[8 * k + 4];

@@ -420,12 +420,9 @@ FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
 // most four of parts): 64 + 20 times 2^-24; what q's parts leave out is 2^-23 of a
 // value, or 2^-25 of the head's largest where a remainder is subnormal.
 //
-// q is scaled by powers of two, its largest value to [1, 2) for f16, to 2^-12 of
-// that for bf16, whose bounds may be as large as an f32: no sum of 2 D products
-// overflows then (2^9 x 2^-11 x the largest).  At the other end a product may be
-// lost below the least normal f32: 2 D x 3 of them are at most 2^-24 of a head's
-// size with bounds of 10^-26, so E takes no smaller bound; a score itself is
-// rounded at 2^-149, twice, and 2^12 times that: less than 10^-40, which E adds.
+// A product may be lost below the least normal f32: the 3 D that are not zero are
+// less than 2^-24 of a head's size with bounds of 10^-26, so E takes no smaller
+// bound; a score itself is rounded at 2^-149, less than 10^-40, which E adds.
 //
 // Bound by HBM while it scores (4 D bytes a page), by barriers and single steps
 // while it chooses: 16 sequences of up to 2,048 pages and 4 KV heads, 94 MB, 33.2
@@ -439,7 +436,6 @@ template <class T, int D, int GP>
 __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a, uint32_t slice, uint32_t together) {
   constexpr int STEPS = D / 8, NT = (Parts<T>::N * GP + 7) / 8;        // 16-product steps a page; column tiles
   constexpr uint32_t STAGES = D / 32;                                  // stages (4 steps) a tile of 16 pages
-  constexpr float kUp = T::kType == FZ_KV_F16 ? 1.f : 4096.f, kDown = 1.f / kUp;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Shared sh;
   __shared__ float norm[8], scale[8], bound[kThreads / 32];
@@ -468,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
   const uint32_t s = (uint32_t)(item / v.kv_heads), h = (uint32_t)(item % v.kv_heads);
   const float* q = a.q + s * a.q_stride + (size_t)h * G * D;
   const uint32_t length = v.lengths[s];
-  // q: each head's size and scale (the largest to [1, 2)).
+  // q: each head's size and scale.
   if (warp < GP) {
     float sum = 0.f, top = 0.f;
     for (int i = lane; i < D / 4 && warp < (int)G; i += 32) {
@@ -477,8 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
       top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
     }
     sum = warp_sum(sum), top = warp_max(top);
-    const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);   // 2^(e - 127) <= top
-    if (lane == 0) norm[warp] = 88.f * sum + top * (D / 2), scale[warp] = top == INFINITY ? NAN : __uint_as_float((uint32_t)e << 23);
+    if (lane == 0) norm[warp] = 88.f * sum + top * (D / 2), scale[warp] = top == INFINITY ? NAN : __uint_as_float(query_exponent<T>(top) << 23);
   }
   const uint32_t entries = min(length, v.table_stride * v.page_slots);
   if (t == 0 && rank == 0 && length > entries) note(v, FZ_PAGED_BAD_LENGTH);
@@ -539,8 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
       const bool least = at < D;
       const float y[4] = {(x.x < 0.f) == least ? x.x : x.x * 0.f, (x.y < 0.f) == least ? x.y : x.y * 0.f,
                           (x.z < 0.f) == least ? x.z : x.z * 0.f, (x.w < 0.f) == least ? x.w : x.w * 0.f};
-      const Parts<T> p0 = parts<T>(y[0] * down * kDown, y[1] * down * kDown),
-                     p1 = parts<T>(y[2] * down * kDown, y[3] * down * kDown);
+      const Parts<T> p0 = parts<T>(y[0] * down, y[1] * down), p1 = parts<T>(y[2] * down, y[3] * down);
 #pragma unroll
       for (int c = 0; c < NT; c++)
         qf[(k * NT + c) * 32 + lane] = GP == 8 ? make_uint2(p0.w[c], p1.w[c])
@@ -593,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
 #pragma unroll
       for (int c = 1; c < NT; c++) x += sum[c][2 * r], y += sum[c][2 * r + 1];
       if (GP == 4) x += __shfl_xor_sync(0xffffffffu, x, 2), y += __shfl_xor_sync(0xffffffffu, y, 2);
-      best[r] = max(has0 ? order(x * c0 * kUp) : 0u, has1 ? order(y * c1 * kUp) : 0u);
+      best[r] = max(has0 ? order(x * c0) : 0u, has1 ? order(y * c1) : 0u);
       best[r] = max(best[r], __shfl_xor_sync(0xffffffffu, best[r], 1));
       if (GP == 8) best[r] = max(best[r], __shfl_xor_sync(0xffffffffu, best[r], 2));
       const uint32_t i = tile * 16 + g4 + 8 * r, page = __shfl_sync(0xffffffffu, mine, g4 + 8 * r);

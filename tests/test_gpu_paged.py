@@ -467,6 +467,23 @@ def test_attention_selected_bad_blocks():
         assert int(cache.error) == bit, words
 
 
+@pytest.mark.parametrize("q_scale", [1e-38, 1e-5, 1e-2])
+def test_attention_largest_bf16_keys(q_scale):
+    """Keys about the largest f32 and queries that leave the scores in range: a head whose products all have one sign."""
+    torch = torch_cuda()
+    cache = Cache([500], page=16, d=256, type="bf16")
+    p, o = cache.at(0, [17])
+    cache.keys[p, o, 0] = 3.3e38
+    q = randn(1, 4, 256, seed=8).abs().clamp(0.5, 2.0) * q_scale
+    q[0, 1] *= -1.0                                                   # the key's score far below the others' at 1e-2
+    scale = 1e-4
+    got = attend(cache, q, scale)
+    want, _, _ = attend_exact(cache, q, scale)
+    # the key's weight is 0 or 1, or every score's products sum to less than 0.2: delta <= 264 2^-24 0.2
+    bound = cache.values.double().abs().max() * (2 * 264 * 0.2 + 500 + 64) * 2.0 ** -24
+    assert ((got.double() - want).abs() <= bound).all()
+
+
 def test_attention_peaky_tiny_and_huge_scores():
     """One key takes nearly all the weight over many small ones; queries of 1e-30 and 1e4; keys of the type's largest values."""
     torch = torch_cuda()
