@@ -30,7 +30,7 @@ struct AttendArgs {
   float2* part_ml;         // [kCtas][2][8] their maximum and sum
   uint4* heads;            // [kCtas] the split item a CTA begins: {item, CTAs, its slot, 0}
   uint4* origin;           // [items] where an item's outputs are, for the weights: {first CTA, CTAs, its slot, 0}
-  float2* stats;           // [items][8] an unsplit item's maximum and reciprocal sum, for the weights
+  float2* stats;           // [items][8] an unsplit item's maximum and reciprocal sum of weights, for the weights
   float* scores;           // [items][group][score_stride] in log2 units, for the weights
   uint64_t score_stride;
 };
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   constexpr int NT = (TERMS * GP + 7) / 8;         // column tiles
   constexpr int CHAINS = 4 / MS;                   // independent sums a score
   constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte pieces a row, rows a copy step
-  constexpr float kShift = T::kType == FZ_KV_F16 ? 15.f : 0.f;
+  constexpr float kShift = T::kType == FZ_KV_F16 ? 15.f : 0.f, kUnit = T::kType == FZ_KV_F16 ? 32768.f : 1.f;   // 2^kShift
   constexpr float kLift = T::kType == FZ_KV_F16 ? 2048.f : 1.f;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ float2 ml[kWarps][8];
@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
           const float inv = sum == 0.f ? 0.f : 1.0f / sum;
           *reinterpret_cast<float4*>(a.out + seg.s * a.out_stride + (seg.h * (size_t)G + g) * D + r * DR + d) =
               make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-          if (v.weights && r == 0 && d == 0) a.stats[item * 8 + g] = make_float2(sum == 0.f ? 0.f : top - kShift, inv);
+          if (v.weights && r == 0 && d == 0) a.stats[item * 8 + g] = make_float2(sum == 0.f ? 0.f : top, inv * kUnit);
         } else {
           *reinterpret_cast<float4*>(a.part_o + ((size_t)part * G + g) * D + r * DR + d) = x;
           if (r == 0 && d == 0) a.part_ml[part * 8 + g] = make_float2(top, sum);
@@ -689,13 +689,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
 // in a fixed order, so the sum never depends on who came first.
 //
 // The others make the entries' weights from the scores and the items' maxima
-// and sums, 128 entries a warp at a time, four a lane, each entry written by the
+// and sums, exp2(score - maximum) / sum (the maximum as it is: one shifted by
+// the f16 weights' 2^15 would be rounded from 2^24 on), 128 entries a warp at a time, four a lane, each entry written by the
 // one lane it falls to.
 constexpr int kWeighed = 128;
 template <int D, bool F16>
 __global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, uint32_t ctas, uint32_t joins, uint32_t pieces) {
   constexpr int COLS = 16, LANES = kThreads / COLS, MOST = (kCtas + LANES - 1) / LANES;
-  constexpr float kShift = F16 ? 15.f : 0.f;
+  constexpr float kUnit = F16 ? 32768.f : 1.f;     // attend_kernel's sums are of weights times this
   __shared__ float factor[kCtas];
   __shared__ float4 sums[kThreads];
   __shared__ float reduce[2][kWarps];
@@ -825,7 +826,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, ui
         sum *= fold(top, upper);
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        m = sum == 0.f ? 0.f : upper - kShift, inv = sum == 0.f ? 0.f : 1.0f / sum;
+        m = sum == 0.f ? 0.f : upper, inv = sum == 0.f ? 0.f : kUnit / sum;
       }
     }
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
