@@ -252,6 +252,15 @@ FZ_DEV uint32_t transpose(uint32_t v) {
 // exp2 of a difference to the maximum of `m`'s side: 0 for a side without entries.
 FZ_DEV float fold(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
 
+// What the softmax weights of a list of `count` entries are multiplied by on the
+// way to the output: f16 ones by 2^15, so that small ones keep their bits, bf16
+// ones by at most 1 / (2 count), so that no partial sum of values about the
+// largest f32 overflows where their average does not.
+template <class T>
+FZ_DEV float unit_of(uint32_t count) {
+  return T::kType == FZ_KV_F16 ? 32768.f : __uint_as_float((94u + __clz(count - 1)) << 23);
+}
+
 // softmax(q k / sqrt d) v for one query a head over a paged list of entries.
 //
 // The products run on mma.sync m16n8k16 with the entries in the M axis and the
@@ -261,8 +270,8 @@ FZ_DEV float fold(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - 
 // accuracy comes from the 8 columns: with 4 heads or fewer they hold the heads'
 // f16 parts and remainders side by side (GP = 4, one MMA a step for f16); with
 // more (GP = 8) one MMA a part.  q is scaled by a power of two a head, so its
-// parts keep 22 bits whatever its size, f16 weights by 2^15 and their remainders
-// by 2^11 more, so that many small ones still sum (to 2^-51 of the largest).  A
+// parts keep 22 bits whatever its size, the remainders of the f16 weights by 2^11
+// more than unit_of, so that many small ones still sum (to 2^-51 of the largest).  A
 // tile's product starts from zero and is added to the running output in f32 (the
 // fold's multiply-add), so the tensor cores' own accumulation never runs along
 // the sequence.
@@ -291,7 +300,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   constexpr int NT = (TERMS * GP + 7) / 8;         // column tiles
   constexpr int CHAINS = 4 / MS;                   // independent sums a score
   constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte pieces a row, rows a copy step
-  constexpr float kShift = T::kType == FZ_KV_F16 ? 15.f : 0.f, kUnit = T::kType == FZ_KV_F16 ? 32768.f : 1.f;   // 2^kShift
   constexpr float kLift = T::kType == FZ_KV_F16 ? 2048.f : 1.f;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ float2 ml[kWarps][8];
@@ -491,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
     Walk after = seg;
     const bool then = next(a, after, KT, extra);
     if (then && mine(after)) ask_q(after);
-    const float c0 = qc[(2 * t4) % GP], c1 = qc[(2 * t4 + 1) % GP];
+    const float c0 = qc[(2 * t4) % GP], c1 = qc[(2 * t4 + 1) % GP], unit_w = unit_of<T>(seg.l.count);
     float o[KS][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
     for (int k = 0; k < KS; k++)
@@ -574,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
       for (int ms = 0; ms < MS; ms++)
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          const float p0 = exp2f(s[ms][2 * i] - b0 + kShift), p1 = exp2f(s[ms][2 * i + 1] - b1 + kShift);
+          const float p0 = exp2f(s[ms][2 * i] - b0) * unit_w, p1 = exp2f(s[ms][2 * i + 1] - b1) * unit_w;
           l0 += p0, l1 += p1;
           const Parts<T> p = parts<T>(p0, p1, kLift);
 #pragma unroll
@@ -662,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
           const float inv = sum == 0.f ? 0.f : 1.0f / sum;
           *reinterpret_cast<float4*>(a.out + seg.s * a.out_stride + (seg.h * (size_t)G + g) * D + r * DR + d) =
               make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-          if (v.weights && r == 0 && d == 0) a.stats[item * 8 + g] = make_float2(sum == 0.f ? 0.f : top, inv * kUnit);
+          if (v.weights && r == 0 && d == 0) a.stats[item * 8 + g] = make_float2(sum == 0.f ? 0.f : top, inv * unit_w);
         } else {
           *reinterpret_cast<float4*>(a.part_o + ((size_t)part * G + g) * D + r * DR + d) = x;
           if (r == 0 && d == 0) a.part_ml[part * 8 + g] = make_float2(top, sum);
@@ -689,14 +697,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
 // in a fixed order, so the sum never depends on who came first.
 //
 // The others make the entries' weights from the scores and the items' maxima
-// and sums, exp2(score - maximum) / sum (the maximum as it is: one shifted by
-// the f16 weights' 2^15 would be rounded from 2^24 on), 128 entries a warp at a time, four a lane, each entry written by the
-// one lane it falls to.
+// and sums, exp2(score - maximum) / sum (the maximum as it is: one
+// lifted with the weights' unit would be rounded from 2^24 on), 128 entries a warp at a time, four a lane, each entry written by the
+// one lane it falls to.  (Without the bound on the CTAs an SM some forms were
+// compiled to 80 registers and spilled: 10.8 -> 11.2 us for 2,048 selected entries
+// of 8 sequences.)
 constexpr int kWeighed = 128;
-template <int D, bool F16>
-__global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, uint32_t ctas, uint32_t joins, uint32_t pieces) {
+template <class T, int D>
+__global__ void __launch_bounds__(kThreads, 2) finish_kernel(const AttendArgs a, uint32_t ctas, uint32_t joins, uint32_t pieces) {
   constexpr int COLS = 16, LANES = kThreads / COLS, MOST = (kCtas + LANES - 1) / LANES;
-  constexpr float kUnit = F16 ? 32768.f : 1.f;     // attend_kernel's sums are of weights times this
   __shared__ float factor[kCtas];
   __shared__ float4 sums[kThreads];
   __shared__ float reduce[2][kWarps];
@@ -826,7 +835,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const AttendArgs a, ui
         sum *= fold(top, upper);
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        m = sum == 0.f ? 0.f : upper, inv = sum == 0.f ? 0.f : kUnit / sum;
+        m = sum == 0.f ? 0.f : upper, inv = sum == 0.f ? 0.f : unit_of<T>(l.count) / sum;
       }
     }
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -855,11 +864,11 @@ template <class T>
 const void* attend_of(uint32_t d, uint32_t group) {
   return d == 64 ? attend_of<T, 64>(group) : d == 128 ? attend_of<T, 128>(group) : attend_of<T, 256>(group);
 }
-template <bool F16>
+template <class T>
 const void* finish_of(uint32_t d) {
-  return d == 64    ? (const void*)finish_kernel<64, F16>
-         : d == 128 ? (const void*)finish_kernel<128, F16>
-                    : (const void*)finish_kernel<256, F16>;
+  return d == 64    ? (const void*)finish_kernel<T, 64>
+         : d == 128 ? (const void*)finish_kernel<T, 128>
+                    : (const void*)finish_kernel<T, 256>;
 }
 
 // Where each part of the workspace begins; returns its whole size.
@@ -956,5 +965,5 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   if (a.kv.weights) weighs = (uint32_t)std::min<uint64_t>(8 * kCtas, (items * pieces + kWarps - 1) / kWarps);
   if (!joins && !weighs) return FZ_OK;
   void* left[] = {&a, &ctas, &joins, &pieces};
-  return paged_launch(f16 ? finish_of<true>(d) : finish_of<false>(d), dim3(joins + weighs), dim3(kThreads), 0, 1, left, stream);
+  return paged_launch(f16 ? finish_of<F16>(d) : finish_of<Bf16>(d), dim3(joins + weighs), dim3(kThreads), 0, 1, left, stream);
 }

@@ -48,3 +48,30 @@ def test_weights_at_large_scores(type, score, heads, lengths):
         # (the scores are equal, so the output's error is the weights')
         bound = cache.rows(cache.values, s, np.arange(n), 0).abs().max() * (n + 64) * 2.0 ** -24
         assert ((got[s].double() - want[s]).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("size", [3.3895e38, 1e38, 1.0, 1e-30])
+@pytest.mark.parametrize("heads,d,lengths,alike", [
+    (4, 256, [1, 2, 3, 16, 300], True), (8, 128, [5000, 2, 70], True), (3, 64, [40000], True), (4, 256, [9000, 33], False),
+    (16, 64, [500] * 20, False)])
+def test_bf16_values_of_any_size(size, heads, d, lengths, alike):
+    """Values about the largest bf16 (an average of them is no larger) and about the least: `alike`, one key and one
+    value a sequence, so that every partial sum grows with the entries; else random ones."""
+    torch = torch_cuda()
+    kv = heads // 8 or 1
+    cache = Cache(lengths, page=16, kv=kv, d=d, type="bf16", weights=True, seed=d)
+    if alike:
+        cache.keys.fill_(0.5)
+        sign = torch.where(torch.arange(d, device="cuda") % 3 == 0, -1.0, 1.0)
+        cache.values.copy_((sign * size).to(cache.dtype).expand_as(cache.values))
+    else:
+        v = cache.values.float().clamp(-1.0, 1.0) * size
+        cache.values.copy_(v)
+    q = randn(len(lengths), heads, d, seed=3)
+    got = attend(cache, q, d ** -0.5)
+    want, weights, bound = attend_exact(cache, q, d ** -0.5)
+    assert torch.isfinite(got).all()
+    assert ((got.double() - want).abs() <= bound).all()
+    for (s, h), (j, w) in weights.items():
+        p, o = cache.at(s, j)
+        assert ((cache.weights[p, h, o].double() - w).abs() <= w * 1e-3).all()
