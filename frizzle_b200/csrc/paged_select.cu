@@ -104,7 +104,7 @@ struct Threshold {
   bool none, every;        // no free key is taken; all are
 };
 
-// `keys[0 .. n)`: this CTA's, of indices first ..; `forced(index)` ones are
+// `keys[0 .. n)`: this CTA's, of indices first ..; `forced(index, key)` ones are
 // taken beforehand and count to `take`.  The digits, 9 bits each, begin at the
 // highest bit in which the keys differ, so that scores of like size take one
 // or two.
@@ -118,11 +118,12 @@ FZ_DEV Threshold<K> find(const Group& group, Shared& sh, const K* keys, uint32_t
   uint32_t pinned = 0;
   K least = ~(K)0, most = 0;
   for (uint32_t i = t; i < n; i += kThreads) {
-    if (forced(first + i)) {
+    const K k = keys[i];
+    if (forced(first + i, k)) {
       pinned++;
     } else {
-      least = keys[i] < least ? keys[i] : least;
-      most = keys[i] > most ? keys[i] : most;
+      least = k < least ? k : least;
+      most = k > most ? k : most;
     }
   }
   pinned = __reduce_add_sync(0xffffffffu, pinned);
@@ -177,7 +178,7 @@ FZ_DEV Threshold<K> find(const Group& group, Shared& sh, const K* keys, uint32_t
     uint32_t* bins = sh.bins[digit & 1];
     for (uint32_t i = t; i < n; i += kThreads) {
       const K k = keys[i];
-      if ((k & r.mask) == r.prefix && !forced(first + i)) atomicAdd(&bins[(uint32_t)(k >> shift) & digits], 1u);
+      if ((k & r.mask) == r.prefix && !forced(first + i, k)) atomicAdd(&bins[(uint32_t)(k >> shift) & digits], 1u);
     }
     sync(group);
     // Thread t: a bin from the top, summed over the cluster.  Every CTA does so: telling the others what one found
@@ -213,7 +214,7 @@ FZ_DEV Threshold<uint32_t> find_alone(Shared& sh, const uint32_t* keys, uint32_t
   uint32_t pinned = 0, least = ~0u, most = 0;
   for (uint32_t i = t; i < n; i += kThreads) {
     const uint32_t k = keys[i];
-    if (forced(i)) pinned++;
+    if (forced(i, k)) pinned++;
     else least = min(least, k), most = max(most, k);
   }
   pinned = __reduce_add_sync(0xffffffffu, pinned);
@@ -247,7 +248,7 @@ FZ_DEV Threshold<uint32_t> find_alone(Shared& sh, const uint32_t* keys, uint32_t
     const uint32_t digits = (1u << bits) - 1;
     for (uint32_t i = t; i < n; i += kThreads) {
       const uint32_t k = keys[i];
-      if ((k & r.mask) == r.prefix && !forced(i)) atomicAdd(&bins[(k >> shift) & digits], 1u);
+      if ((k & r.mask) == r.prefix && !forced(i, k)) atomicAdd(&bins[(k >> shift) & digits], 1u);
     }
     __syncthreads();
     if (warp == 0) {
@@ -329,7 +330,7 @@ FZ_DEV Range<K> range_of(const Threshold<K>& r) {
 // The entries taken beforehand: the first `sink` of n and the last `recent`.
 struct Forced {
   uint32_t sink, tail;
-  FZ_DEV bool operator()(uint32_t i) const { return i < sink || i >= tail; }
+  FZ_DEV bool operator()(uint32_t i, uint32_t = 0) const { return i < sink || i >= tail; }
 };
 FZ_DEV Forced forced_of(uint32_t n, uint32_t sink, uint32_t recent) { return Forced{sink, n > recent ? n - recent : 0u}; }
 
@@ -698,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
   }
   if (!refine) return;
   // The near pages in f64, a CTA its own; the rest of the choice is made.
-  auto taken_first = [&](uint32_t i) { return forced(i) || near_t.side(keys[i - first]) == 2; };
+  auto taken_first = [&](uint32_t i, uint64_t = 0) { return forced(i) || near_t.side(keys[i - first]) == 2; };
   for (uint32_t i = warp; i < n; i += kThreads / 32) {
     double d = 0.0;
     const bool near = !forced(first + i) && near_t.side(keys[i]) == 1;
@@ -743,8 +744,8 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const EvictArgs a, uint3
   const uint32_t entries = held(v, s);
   if (threadIdx.x == 0 && rank == 0 && v.lengths[s] > entries) note(v, FZ_PAGED_BAD_LENGTH);
   uint32_t* out = a.kept + item * a.budget;
-  for (uint32_t i = min(entries, a.budget) + rank * kThreads + threadIdx.x; i < a.budget; i += size * kThreads)
-    out[i] = FZ_PAGED_NONE;
+  // (A barrier of the choice lies between these and the entries taken.)
+  for (uint32_t i = rank * kThreads + threadIdx.x; i < a.budget; i += size * kThreads) out[i] = FZ_PAGED_NONE;
   const uint32_t per = (entries + size - 1) / size, first = min(entries, rank * per), n = min(entries, first + per) - first;
   const uint32_t* table = v.table + (size_t)s * v.table_stride;
   for (uint32_t i0 = threadIdx.x; i0 < n; i0 += BATCH * kThreads) {
@@ -771,13 +772,18 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const EvictArgs a, uint3
   }
   __syncthreads();
   cluster.barrier_wait();
-  const Forced forced = forced_of(entries, a.sink, a.recent);
+  // (Entries of pages that are none, key 0, are not forced, chosen last and never taken.)
+  const Forced ends = forced_of(entries, a.sink, a.recent);
+  auto forced = [&](uint32_t i, uint32_t key) { return ends(i) && key; };
   const Group group = size == 1 ? Group{nullptr, 1, 0} : Group{&cluster, size, rank};
   const Threshold<uint32_t> r = size == 1 ? find_alone(sh, keys, n, min(a.budget, entries), forced)
                                           : find(group, sh, keys, n, first, min(a.budget, entries), forced);
   const Range<uint32_t> cut = range_of(r);
   emit_taken(
-      group, sh, n, r.ties, [&](uint32_t i) { return forced(first + i) ? 2 : cut.side(keys[i]); },
+      group, sh, n, r.ties, [&](uint32_t i) {
+        const uint32_t k = keys[i];
+        return !k ? 0 : ends(first + i) ? 2 : cut.side(k);
+      },
       [&](uint32_t i, uint32_t at) { out[at] = first + i; });
 }
 

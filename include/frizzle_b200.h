@@ -584,11 +584,13 @@ size_t fz_paged_attention_workspace(const fz_paged_kv *kv, uint32_t heads);
  * own table; none of them a page `from` holds): the first `sink` and the last
  * `recent` entries first (sink + recent <= budget), then the largest
  * accumulated weights, equal ones by the lower index, NaN before all numbers.
- * Keys, values and weights are copied bit for bit, keys keeping the rotation
- * of the position they were appended at; to->lengths[s] =
- * min(from->lengths[s], budget), and kept[s][h] = the source index of each
- * entry kept, FZ_PAGED_NONE past them ([sequences][kv_heads][budget]).  `from`
- * is left as it was.  A window then counts kept entries. */
+ * Entries of a page that is none are left out, forced or not, so that every
+ * slot `to` holds is written.  Keys, values and weights are copied bit for bit,
+ * keys keeping the rotation of the position they were appended at;
+ * to->lengths[s] = the entries kept, min(from->lengths[s], budget) where all
+ * pages are some, and kept[s][h] = the source index of each, FZ_PAGED_NONE past
+ * them ([sequences][kv_heads][budget]).  `from` is left as it was.  A window
+ * then counts kept entries. */
 fz_status fz_paged_evict(const fz_paged_kv *from, const fz_paged_kv *to, uint32_t budget, uint32_t sink,
                          uint32_t recent, uint32_t *kept, void *stream);
 

@@ -75,3 +75,46 @@ def test_bf16_values_of_any_size(size, heads, d, lengths, alike):
     for (s, h), (j, w) in weights.items():
         p, o = cache.at(s, j)
         assert ((cache.weights[p, h, o].double() - w).abs() <= w * 1e-3).all()
+
+
+# ------------------------------------------------------------------ eviction
+
+@pytest.mark.parametrize("kv,lengths,bad,budget,sink,recent", [
+    (1, [64], [0], 48, 4, 8), (2, [64, 50], [3, 0], 64, 0, 0), (1, [64], [0, 3], 20, 20, 0), (1, [64], [1, 3], 20, 0, 20),
+    (2, [64, 3, 0], [0, 1, 2, 3], 64, 5, 5), (1, [20000, 100], [0, 700, 1249], 15000, 30, 30),
+    (1, [20000, 64], [0, 700, 1249], 20000, 0, 0), (3, [9000], [562, 3], 9000, 16, 16), (1, [6000], [5], 100, 90, 10)])
+def test_evict_leaves_out_entries_of_bad_pages(kv, lengths, bad, budget, sink, recent):
+    """Logical pages `bad` of every sequence are no pages: what they hold is left out even where it is forced or the
+    budget has room for it, so that every slot the new cache holds was written."""
+    torch = torch_cuda()
+    a = Cache(lengths, page=16, kv=kv, d=64, weights=True, seed=1)
+    b = Cache([max(1, min(n, budget)) for n in lengths], page=16, kv=kv, d=64, weights=True, seed=2, fill=float("nan"))
+    b.weights.fill_(float("nan"))
+    b.len.fill_(77)
+    table = u32(a.table).copy()
+    table[:, [i for i in bad if i < table.shape[1]]] = a.pages + 5
+    words = Cache.u32(table)
+    a.desc.page_table = words.data_ptr()
+    kept = u32(evict(a, b, budget, sink, recent))
+    new = []
+    for s, n in enumerate(lengths):
+        good = np.array([i for i in range(n) if i // 16 not in bad], dtype=np.int64)
+        take = min(budget, len(good))
+        new.append(take)
+        for h in range(kv):
+            w = a.weight(s, good, h).double().cpu().numpy() if len(good) else np.zeros(0)
+            forced = (good < sink) | (good + recent >= n)
+            want = np.sort(good[np.lexsort((good, -w, ~forced))[:take]])
+            assert np.array_equal(kept[s, h, :take], want), (s, h)
+            assert (kept[s, h, take:] == NONE).all()
+            if take:
+                (p, o), (tp, to) = a.at(s, want), b.at(s, np.arange(take))
+                assert (b.keys[tp, to, h] == a.keys[p, o, h]).all() and (b.values[tp, to, h] == a.values[p, o, h]).all()
+                assert (b.weights[tp, h, to] == a.weights[p, h, o]).all()
+    assert list(u32(b.len)) == new
+    assert int(b.error) == 0 and int(a.error) == (1 if any(i * 16 < n for i in bad for n in lengths) else 0)
+    q = randn(len(lengths), kv, 64)
+    b.lengths = new
+    got = attend(b, q, 0.125)
+    want, _, bound = attend_exact(b, q, 0.125)
+    assert ((got.double() - want).abs() <= bound).all()
