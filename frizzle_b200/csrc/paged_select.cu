@@ -386,6 +386,121 @@ FZ_DEV double page_score(const SelectArgs& a, const float* q, uint32_t page, uin
   return best;
 }
 
+// A finite value of a 16-bit type as f64 times 2^-896: the exponent and leading
+// bits of its f32 moved to f64's upper word (the lower one is zero), subnormal or
+// not, by two integer instructions; a conversion runs at a fraction of their rate.
+FZ_DEV uint32_t upper_word(float x) { return (uint32_t)((int)__float_as_uint(x) >> 3) & 0x8FFFFFFFu; }
+
+// The greater sizes of two pairs, NaN kept; and whether one of a pair is no
+// finite value.
+template <class T>
+FZ_DEV uint32_t greatest_size(uint32_t m, uint32_t x);
+template <>
+FZ_DEV uint32_t greatest_size<F16>(uint32_t m, uint32_t x) {
+  const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&m), __habs2(*reinterpret_cast<__half2*>(&x)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <>
+FZ_DEV uint32_t greatest_size<Bf16>(uint32_t m, uint32_t x) {
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&m), __habs2(*reinterpret_cast<__nv_bfloat162*>(&x)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <class T>
+FZ_DEV bool not_finite(uint32_t word) {
+  constexpr bool F = T::kType == FZ_KV_F16;
+  return ((word & (F ? 0x7C007C00u : 0x7F807F80u)) + (F ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+}
+
+// q's values as f64 times 2^126, for a lane to read its eight of a head two at a
+// time without bank conflicts: where value i of head g lies.
+template <int D>
+FZ_DEV uint32_t lifted_place(uint32_t g, uint32_t i) {
+  return ((g * 4 + i % 8 / 2) * (D / 8) + i / 8) * 2 + i % 2;
+}
+constexpr int kLift = 126;               // (sums of products are times 2^-770 then, which keeps all that f32 could hold)
+
+// The scores of the listed pages as their f64 sums rounded to f32 (rounding
+// keeps the order, so the largest of the heads is taken of the rounded ones):
+// D / 8 lanes a page and 16 bytes of each row a lane.  A page with an infinity or
+// NaN by page_score.  Bound by the instructions of 16 warps an SM: 128 pages by 8
+// SMs cost a selection of 2,032 pages 2.4 us, 200 pages by two of 16 x 4 7.0 (all
+// by page_score 2.8 and 15; q's parts in registers instead of shared memory 3.6
+// and 6.2, eight lanes a page 3.3 and 6.0).
+template <class T, int D, int GP>
+FZ_DEV void listed_scores(const SelectArgs& a, const float* q, const double* lifted, uint32_t h, const uint32_t* table,
+                          const uint32_t* list, float* scores, uint32_t take, uint32_t w, uint32_t warps) {
+  constexpr uint32_t LANES = D / 8, PER = 32 / LANES;                  // lanes a page, pages a step
+  const uint32_t lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES;
+  const double2* x = reinterpret_cast<const double2*>(lifted) + part;
+  const double back = __hiloint2double((1023 - kLift + 896) << 20, 0);
+  for (uint32_t base = PER * w; base < take; base += 32 * warps) {
+    // Lane l: the word of entry l mod PER of step l / PER.
+    const uint32_t mine = base + lane / PER * PER * warps + lane % PER;
+    const uint32_t words = mine < take ? table[__ldcg(list + mine)] : FZ_PAGED_NONE;
+    const uint32_t steps = min(LANES, (take - base + PER * warps - 1) / (PER * warps));
+    uint4 lo, hi;
+    auto load = [&](uint32_t step) {
+      const uint32_t page = __shfl_sync(0xffffffffu, words, PER * step + sub), at = page < a.kv.pages ? page : 0u;
+      const uint4* b = reinterpret_cast<const uint4*>(a.kv.bounds + ((size_t)at * a.kv.kv_heads + h) * 2 * D) + part;
+      lo = b[0], hi = b[LANES];
+      return page;
+    };
+    uint32_t next = load(0);
+#pragma unroll 1
+    for (uint32_t step = 0; step < steps; step++) {
+      const uint32_t l4[4] = {lo.x, lo.y, lo.z, lo.w}, u4[4] = {hi.x, hi.y, hi.z, hi.w}, page = next;
+      if (step + 1 < steps) next = load(step + 1);
+      uint32_t l[8], u[8], most = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float2 y = T::unpack(l4[i]), z = T::unpack(u4[i]);
+        l[2 * i] = upper_word(y.x), l[2 * i + 1] = upper_word(y.y);
+        u[2 * i] = upper_word(z.x), u[2 * i + 1] = upper_word(z.y);
+        most = greatest_size<T>(greatest_size<T>(most, l4[i]), u4[i]);
+      }
+      // Two heads' chains at once (the second of an odd number is zeros).
+      double s[GP];
+#pragma unroll
+      for (int g = 0; g < GP; g++) s[g] = 0.0;
+#pragma unroll
+      for (int g = 0; g < GP; g += 2)
+        if (g < (int)a.group) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int k = g; k < g + 2; k++) {
+              const double2 y = x[(k * 4 + i) * LANES];
+              s[k] = fma(y.x, __hiloint2double(__double2hiint(y.x) < 0 ? l[2 * i] : u[2 * i], 0), s[k]);
+              s[k] = fma(y.y, __hiloint2double(__double2hiint(y.y) < 0 ? l[2 * i + 1] : u[2 * i + 1], 0), s[k]);
+            }
+        }
+      // Half the heads to half the lanes at each step, until a lane has one.
+      uint32_t head = 0;
+      int o = LANES / 2;
+#pragma unroll
+      for (int n = GP / 2; n > 0; n /= 2, o /= 2) {
+        const bool upper = lane & o;
+        head += upper ? n : 0;
+#pragma unroll
+        for (int i = 0; i < n; i++) s[i] = (upper ? s[i + n] : s[i]) + __shfl_xor_sync(0xffffffffu, upper ? s[i] : s[i + n], o);
+      }
+#pragma unroll
+      for (; o > 0; o /= 2) s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+      uint32_t best = head < a.group ? order((float)(s[0] * back)) : 0u;
+#pragma unroll
+      for (o = LANES / 2; o > (int)LANES / 2 / GP; o /= 2) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+      for (uint32_t left = __ballot_sync(0xffffffffu, not_finite<T>(most)); left;) {
+        const uint32_t first = (__ffs(left) - 1) / LANES * LANES, at = __shfl_sync(0xffffffffu, page, first);
+        const uint32_t key = order((float)page_score<T, D>(a, q, at < a.kv.pages ? at : 0u, h, lane));
+        if (sub == first / LANES) best = key;
+        left &= ~((LANES == 32 ? ~0u : (1u << LANES % 32) - 1) << first);
+      }
+      const uint32_t e = base + step * PER * warps + sub;
+      if (part == 0 && e < take) scores[e] = page < a.kv.pages ? __uint_as_float(topk_bits(best)) : -INFINITY;
+    }
+  }
+}
+
 template <class T>
 FZ_DEV uint32_t greater_size(uint32_t m, uint32_t x);
 template <>
@@ -426,9 +541,10 @@ FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
 // bound; a score itself is rounded at 2^-149, less than 10^-40, which E adds.
 //
 // Bound by HBM while it scores (4 D bytes a page), by barriers and single steps
-// while it chooses: 16 sequences of up to 2,048 pages and 4 KV heads, 94 MB, 33.2
+// while it chooses: 16 sequences of up to 2,048 pages and 4 KV heads, 94 MB, 32.8
 // us, 22 of them scoring the longest (all in f64: 90 us; f32 lanes and shuffles:
-// 61); one sequence of 2,032 pages 15.0 us (59, 25.7).
+// 61); one sequence of 2,032 pages 14.8 us (59, 25.7).  With the listed pages'
+// scores, which are f64's again, 39.8 and 17.2 us.
 //
 // Where one CTA's shared memory holds all the cluster's scores (`together`), the
 // first CTA gets them all and chooses alone, two cluster barriers in all; beyond
@@ -612,6 +728,15 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
   if (alone) cluster.sync();
   else __syncthreads();
 
+  // q again, for the listed pages' scores (asked for here, needed after the choice).
+  constexpr int QN = (GP * D + kThreads - 1) / kThreads;
+  float again[QN];
+#pragma unroll
+  for (int i = 0; i < QN; i++) {
+    const uint32_t at = t + i * kThreads;
+    again[i] = scores && at < G * D ? __ldcg(q + at) : 0.f;
+  }
+
   // The threshold among them, by the first CTA alone or by all (their first
   // barrier makes the bounds seen).
   const uint32_t take = min(a.top, pages);
@@ -686,10 +811,13 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
             const int z = forced(from + i) ? 2 : cut.side(keys[i]);
             return z == 1 && by_bit ? (int)(chosen[i / 32] >> (i % 32) & 1) * 2 : z;
           },
-          [&](uint32_t i, uint32_t at) {
-            out[at] = from + i;
-            if (scores) scores[at] = __uint_as_float(topk_bits(keys[i]));
-          });
+          [&](uint32_t i, uint32_t at) { out[at] = from + i; });
+  }
+  double* lifted = reinterpret_cast<double*>(qf);  // (q's operands, 32 D bytes or more a four heads, are done with)
+#pragma unroll
+  for (int i = 0; i < QN; i++) {
+    const uint32_t at = t + i * kThreads;
+    if (at < GP * D) lifted[lifted_place<D>(at / D, at % D)] = (double)again[i] * __hiloint2double((1023 + kLift) << 20, 0);
   }
   if (alone) {
     if (rank == 0 && warp == 0 && t < (int)size)
@@ -697,24 +825,27 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const SelectArgs a,
     cluster.sync();
     refine = sh.verdict.x != 0, near_t = Range<uint32_t>{sh.verdict.y, sh.verdict.z};
   }
-  if (!refine) return;
-  // The near pages in f64, a CTA its own; the rest of the choice is made.
-  auto taken_first = [&](uint32_t i, uint64_t = 0) { return forced(i) || near_t.side(keys[i - first]) == 2; };
-  for (uint32_t i = warp; i < n; i += kThreads / 32) {
-    double d = 0.0;
-    const bool near = !forced(first + i) && near_t.side(keys[i]) == 1;
-    if (near) d = page_score<T, D>(a, q, table[first + i], h, lane);
-    if (lane == 0) exact[i] = near ? order(d) : 0ull;
+  if (refine) {
+    // The near pages in f64, a CTA its own; the rest of the choice is made.
+    auto taken_first = [&](uint32_t i, uint64_t = 0) { return forced(i) || near_t.side(keys[i - first]) == 2; };
+    for (uint32_t i = warp; i < n; i += kThreads / 32) {
+      double d = 0.0;
+      const bool near = !forced(first + i) && near_t.side(keys[i]) == 1;
+      if (near) d = page_score<T, D>(a, q, table[first + i], h, lane);
+      if (lane == 0) exact[i] = near ? order(d) : 0ull;
+    }
+    __syncthreads();
+    const Threshold<uint64_t> r64 = find(whole, sh, exact, n, first, take, taken_first);
+    const Range<uint64_t> cut = range_of(r64);
+    emit_taken(
+        whole, sh, n, r64.ties, [&](uint32_t i) { return taken_first(first + i) ? 2 : cut.side(exact[i]); },
+        [&](uint32_t i, uint32_t at) { out[at] = first + i; });
   }
-  __syncthreads();
-  const Threshold<uint64_t> r64 = find(whole, sh, exact, n, first, take, taken_first);
-  const Range<uint64_t> cut = range_of(r64);
-  emit_taken(
-      whole, sh, n, r64.ties, [&](uint32_t i) { return taken_first(first + i) ? 2 : cut.side(exact[i]); },
-      [&](uint32_t i, uint32_t at) {
-        out[at] = first + i;
-        if (scores) scores[at] = __uint_as_float(topk_bits(keys[i]));
-      });
+  if (!scores) return;
+  // The listed pages' scores, in f64, by all warps.  (A barrier since the list was written; one is past where the
+  // first CTA wrote it alone.)
+  if (refine || !alone) sync(whole);
+  listed_scores<T, D, GP>(a, q, lifted, h, table, out, scores, take, warp * size + rank, size * (kThreads / 32));
 }
 
 // ------------------------------------------------------------ eviction

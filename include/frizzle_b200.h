@@ -545,7 +545,9 @@ fz_status fz_paged_bounds(const fz_paged_kv *kv, const uint32_t *first, void *st
  * last `recent` pages are taken first (sink + recent <= top), then the best
  * scores, equal ones by the lower page, NaN before all numbers.  q as in
  * fz_paged_attention.  scores: NULL or [sequences][kv_heads][top], each
- * chosen page's score in f32 (0 past them).  Keys and values are not read. */
+ * listed page's score rounded to f32 (0 past them; pages that are none come
+ * last, and where one is listed all the same its score is -infinity).  Keys and
+ * values are not read. */
 fz_status fz_paged_select(const fz_paged_kv *kv, const float *q, uint64_t q_stride, uint32_t heads, uint32_t top,
                           uint32_t sink, uint32_t recent, uint32_t *blocks, float *scores, void *stream);
 

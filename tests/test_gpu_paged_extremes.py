@@ -77,6 +77,95 @@ def test_bf16_values_of_any_size(size, heads, d, lengths, alike):
         assert ((cache.weights[p, h, o].double() - w).abs() <= w * 1e-3).all()
 
 
+# ------------------------------------------------------------------ selection
+
+def check_scores(cache, q, blocks, scores, size=None):
+    """Every listed page's score as the 64-bit sum rounded to f32 (half a unit, or half of 2^-149), that sum in any order:
+    (d + 8) 2^-53 of the page's products' sizes."""
+    torch = torch_cuda()
+    blocks, scores = u32(blocks), scores.double().cpu().numpy()
+    G = q.shape[1] // cache.kv
+    for s, n in enumerate(cache.lengths):
+        n = (n + cache.page - 1) // cache.page
+        for h in range(cache.kv):
+            at = blocks[s, h][blocks[s, h] != NONE].astype(np.int64)
+            assert len(at) == min(n, blocks.shape[2]) and (scores[s, h, len(at):] == 0).all()
+            want = page_scores(cache, q, s, h)[at]
+            b = cache.bounds[torch.from_numpy(cache.table_np[s, at].astype(np.int64)).cuda(), h].double()
+            x = q[s, h * G:(h + 1) * G].double()[:, None]
+            sizes = torch.where(x < 0, x * b[:, 0], x * b[:, 1]).abs().sum(-1).amax(0).cpu().numpy()
+            with np.errstate(invalid="ignore", over="ignore"):
+                got, rounded = scores[s, h, :len(at)], want.astype(np.float32).astype(np.float64)
+                near = np.abs(got - want) <= np.abs(want) * 2.0 ** -24 + sizes * (cache.d + 8) * 2.0 ** -53 + 2.0 ** -150
+            same = near | (got == rounded) | (np.isnan(got) & np.isnan(want))
+            assert same.all(), (s, h, got[~same][:4], want[~same][:4])
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("d,heads,kv,page,lengths,top,sink,recent,capacity", [
+    (256, 4, 1, 16, [1000, 0, 1, 16, 700], 12, 1, 2, None), (128, 8, 2, 4, [2000, 1999], 100, 0, 0, None),
+    (64, 15, 3, 8, [300, 50], 64, 3, 5, None), (256, 8, 1, 1, [5000], 257, 4, 4, None), (128, 2, 2, 16, [33, 90], 3, 1, 2, None),
+    (64, 1, 1, 2, [20000], 1, 0, 0, None), (128, 16, 2, 1, [14000], 14000, 0, 9000, None), (256, 8, 4, 16, [9000] * 16, 200, 2, 8, None),
+    (64, 5, 1, 1, [7000, 300], 500, 3, 3, 36000)])
+def test_select_scores_are_the_64_bit_ones(type, d, heads, kv, page, lengths, top, sink, recent, capacity):
+    cache = Cache(lengths, page=page, kv=kv, d=d, type=type, bounds=True, seed=top, capacity=capacity)
+    bounds(cache)
+    q = randn(len(lengths), heads, d, seed=3)
+    check_scores(cache, q, *select(cache, q, top, sink, recent))
+
+
+@pytest.mark.parametrize("pages,take", [(200, 50), (3000, 700), (13000, 5)])
+def test_select_scores_of_near_ties(pages, take):
+    """Scores that f32 sums cannot tell apart, but f32 can hold: 2^13 + k 2^-10."""
+    torch = torch_cuda()
+    cache = Cache([pages * 2], page=2, d=64, bounds=True)
+    k = np.random.default_rng(pages).integers(0, 40, pages)
+    rows = torch.from_numpy(cache.table_np[0].astype(np.int64)).cuda()
+    cache.bounds[rows] = torch.from_numpy(k / 1024.0).cuda().to(cache.dtype)[:, None, None, None]
+    cache.bounds[:, :, :, 0] = 1024.0
+    cache.bounds[:, :, :, 2] = 1000.0
+    q = torch.zeros(1, 1, 64, device="cuda")
+    q[0, 0, 0], q[0, 0, 1], q[0, 0, 2] = 1024.0, 1.0, -1024 * 1.016
+    blocks, scores = select(cache, q, take)
+    check_scores(cache, q, blocks, scores)
+
+
+@pytest.mark.parametrize("heads,lengths", [(2, [40 * 16]), (8, [3000 * 16]), (1, [5 * 16])])
+def test_select_scores_with_bounds_infinite_on_the_side_not_picked(heads, lengths):
+    """q < 0 with a greatest key of inf, q > 0 with a least of -inf: the score is finite."""
+    torch = torch_cuda()
+    cache = Cache(lengths, page=16, d=64, bounds=True)
+    bounds(cache)
+    q = randn(1, heads, 64)
+    q[:, :, 3], q[:, :, 4] = -1.5, 2.0
+    cache.bounds[int(cache.table_np[0, 2]), 0, 1, 3] = float("inf")
+    cache.bounds[int(cache.table_np[0, 4]), 0, 0, 4] = -float("inf")
+    cache.bounds[int(cache.table_np[0, 3]), 0, 1, 4] = float("inf")   # picked: inf
+    for top in (len(cache.table_np[0]), 4):
+        blocks, scores = select(cache, q, top)
+        check_scores(cache, q, blocks, scores)
+    blocks, scores = select(cache, q, 5, 5, 0)
+    check_scores(cache, q, blocks, scores)
+    assert torch.isfinite(scores[0, 0, [2, 4]]).all() and scores[0, 0, 3] == float("inf")
+
+
+@pytest.mark.parametrize("pages,take", [(11, 11), (11, 6), (3000, 40)])
+def test_select_score_of_a_page_that_is_none(pages, take):
+    """-infinity, below every other page's."""
+    cache = Cache([pages * 16], page=16, d=64, bounds=True)
+    bounds(cache)
+    bad = cache.table.clone()
+    bad[0, 1] = bad[0, pages - 2] = -1
+    cache.desc.page_table = bad.data_ptr()
+    q = randn(1, 3, 64)
+    blocks, scores = select(cache, q, take, 2, 3)
+    at = u32(blocks)[0, 0]
+    got = scores[0, 0].cpu().numpy()
+    none = (at == 1) | (at == pages - 2)
+    assert none.sum() == 2 and (got[none] == -np.inf).all() and np.isfinite(got[~none]).all()
+    assert int(cache.error) == 1
+
+
 # ------------------------------------------------------------------ eviction
 
 @pytest.mark.parametrize("kv,lengths,bad,budget,sink,recent", [
