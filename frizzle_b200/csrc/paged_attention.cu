@@ -269,9 +269,13 @@ FZ_DEV float unit_of(uint32_t count) {
 // memory (ldmatrix, transposed for V) and nothing is padded but N.  f32
 // accuracy comes from the 8 columns: with 4 heads or fewer they hold the heads'
 // f16 parts and remainders side by side (GP = 4, one MMA a step for f16); with
-// more (GP = 8) one MMA a part.  q is scaled by a power of two a head, so its
-// parts keep 22 bits whatever its size, the remainders of the f16 weights by 2^11
-// more than unit_of, so that many small ones still sum (to 2^-51 of the largest).  A
+// more (GP = 8) one MMA a part.  q is scaled by a power of two a head, f16 parts so
+// that its largest is about 2^14, and the remainders of f16 parts, q's and the
+// weights', are times 2^11 more: q keeps 22 bits down to 2^-28 of a head's largest
+// (one far larger dimension costs the others nothing) and 2^-50 of that below; the
+// weights, at unit_of, 22 bits and 2^-51 of the largest.  (f32's own 24
+// bits would take one MMA more a step; 2^-22 of a score's products' sizes is less
+// than its f32 sum may be off by.)  A
 // tile's product starts from zero and is added to the running output in f32 (the
 // fold's multiply-add), so the tensor cores' own accumulation never runs along
 // the sequence.
@@ -363,8 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
       q_next[r] = f < (int)(G * D / 4) ? __ldcg(q + f) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
-  // Its parts as B operands in shared memory, scaled so that each head's largest
-  // is in [1, 2).
+  // Its parts as B operands in shared memory.
   auto put_q = [&]() {
     constexpr int W = D / 4 < 32 ? D / 4 : 32, PER = D / 4 / W;     // lanes a group, groups a head
 #pragma unroll
@@ -385,13 +388,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
 #pragma unroll
     for (int i = 1; i < PER; i++) top = fmaxf(top, largest[g * PER + i]);
     uint32_t e = query_exponent<T>(top);
+    if (T::kType == FZ_KV_F16) e = max(e, 15u) - 14;   // (the largest in [2^14, 2^15))
     // (With a scale about the largest f32 the room for keys of that size is given up: the factor stays finite.)
     if (T::kType != FZ_KV_F16 && !(__uint_as_float(e << 23) * a.scale_log2e < INFINITY)) e -= 10;
     const float down = __uint_as_float((254 - e) << 23), up = __uint_as_float(e << 23);
     const float2* q = reinterpret_cast<const float2*>(raw) + g * (D / 2) + t4;
     for (int k = warp; k < KS; k += kWarps) {
       const float2 x = q[8 * k], y = q[8 * k + 4];
-      const Parts<T> p0 = parts<T>(x.x * down, x.y * down), p1 = parts<T>(y.x * down, y.y * down);
+      const Parts<T> p0 = parts<T>(x.x * down, x.y * down, kLift), p1 = parts<T>(y.x * down, y.y * down, kLift);
 #pragma unroll
       for (int n = 0; n < NT; n++)
         qf[(k * NT + n) * 32 + lane] = GP == 8 ? make_uint2(p0.w[n], p1.w[n])
@@ -536,9 +540,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
           for (int i = 0; i < 4; i++) {
             float x = 0.f;
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int n = NT - 1; n >= 0; n--) {
+              if (kLift > 1.f && n == 0) x *= 1.f / kLift;
 #pragma unroll
               for (int ch = 0; ch < CHAINS; ch++) x += sc[ms][ch][n][i];
+            }
+            if (kLift > 1.f && GP == 4) x = t4 < 2 ? x : x * (1.f / kLift);
             if (GP == 4) x += __shfl_xor_sync(0xffffffffu, x, 2);
             s[ms][i] = x;
           }

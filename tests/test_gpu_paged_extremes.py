@@ -77,6 +77,20 @@ def test_bf16_values_of_any_size(size, heads, d, lengths, alike):
         assert ((cache.weights[p, h, o].double() - w).abs() <= w * 1e-3).all()
 
 
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,d", [(4, 256), (8, 64), (7, 128)])
+@pytest.mark.parametrize("outlier", [1e4, 1e6, 1e8])
+def test_attention_query_with_one_large_dimension(type, heads, d, outlier):
+    """One dimension far above a head's others, which the keys have at zero: the others count as they do without it."""
+    cache = Cache([1, 30, 700, 3000], page=16, d=d, type=type, seed=heads)
+    cache.keys[..., 5] = 0.0
+    q = randn(4, heads, d, seed=4) * 4.0
+    q[..., 5] = outlier
+    got = attend(cache, q, d ** -0.5)
+    want, _, bound = attend_exact(cache, q, d ** -0.5)
+    assert ((got.double() - want).abs() <= bound).all(), float(((got.double() - want).abs() / bound).max())
+
+
 # ------------------------------------------------------------------ selection
 
 def check_scores(cache, q, blocks, scores, size=None):
