@@ -72,10 +72,12 @@ fz_status paged_view(const fz_paged_kv* kv, uint32_t need, PagedView* out) {
   return FZ_OK;
 }
 
-fz_status paged_launch(const void* kernel, dim3 grid, dim3 block, size_t smem, uint32_t cluster, void** args,
+fz_status paged_launch(const void* kernel, dim3 grid, dim3 block, size_t smem, size_t most, uint32_t cluster, void** args,
                        void* stream) {
   cudaError_t e = cudaSuccess;
-  if (smem > 16 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // (The limit is the function's, for all host threads: always the same one, so that a call with a short table never
+  // lowers it between another's setting and launch.)
+  if (smem > 16 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
@@ -416,7 +418,7 @@ extern "C" fz_status fz_paged_append(const fz_paged_kv* kv, const fz_paged_rows*
   if (blocks > 0x7FFFFFFFull) return paged_refuse(FZ_ERR_ARGUMENT, "too many rows");
   void* args[] = {&a, &warps};
   return paged_launch(many ? pick<AppendManyOf>(kv->type, kv->head_dim) : pick<AppendOf>(kv->type, kv->head_dim),
-                      dim3((uint32_t)blocks), dim3(128), 0, 1, args, stream);
+                      dim3((uint32_t)blocks), dim3(128), 0, 0, 1, args, stream);
 }
 
 extern "C" fz_status fz_paged_bounds(const fz_paged_kv* kv, const uint32_t* first, void* stream) {
@@ -431,6 +433,6 @@ extern "C" fz_status fz_paged_bounds(const fz_paged_kv* kv, const uint32_t* firs
   a.first = first;
   const uint64_t items = (uint64_t)kv->table_stride * kv->kv_heads * kv->sequences;
   void* args[] = {&a};
-  return paged_launch(pick<BoundsOf>(kv->type, kv->head_dim), dim3((uint32_t)std::min<uint64_t>(items, 3 * 148)), dim3(256), 0, 1,
-                      args, stream);
+  return paged_launch(pick<BoundsOf>(kv->type, kv->head_dim), dim3((uint32_t)std::min<uint64_t>(items, 3 * 148)), dim3(256), 0, 0,
+                      1, args, stream);
 }

@@ -140,7 +140,8 @@ fz_status paged_refuse(fz_status s, const char* why);
 // FZ_OK when every pointer (NULL ones left out) is memory the current device
 // reaches as its own; a refusal naming `what` otherwise.
 fz_status paged_on_device(const void* const* pointers, int count, const char* what);
-fz_status paged_launch(const void* kernel, dim3 grid, dim3 block, size_t smem, uint32_t cluster, void** args,
+// `most`: the most dynamic shared memory that any call gives this kernel.
+fz_status paged_launch(const void* kernel, dim3 grid, dim3 block, size_t smem, size_t most, uint32_t cluster, void** args,
                        void* stream);
 
 }  // namespace fz

@@ -964,13 +964,13 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   void* args[] = {&a};
   const bool f16 = kv->type == FZ_KV_F16;
   const uint32_t d = kv->head_dim;
-  if ((st = paged_launch(f16 ? attend_of<F16>(d, a.group) : attend_of<Bf16>(d, a.group), dim3(grid), dim3(kThreads), kSmem, 1,
-                         args, stream)))
+  if ((st = paged_launch(f16 ? attend_of<F16>(d, a.group) : attend_of<Bf16>(d, a.group), dim3(grid), dim3(kThreads), kSmem,
+                         kSmem, 1, args, stream)))
     return st;
   uint32_t joins = a.whole ? 0u : std::min(4 * kCtas, grid * a.group * (d / 64)), weighs = 0, ctas = grid;
   uint32_t pieces = (uint32_t)((most + kWeighed - 1) / kWeighed);
   if (a.kv.weights) weighs = (uint32_t)std::min<uint64_t>(8 * kCtas, (items * pieces + kWarps - 1) / kWarps);
   if (!joins && !weighs) return FZ_OK;
   void* left[] = {&a, &ctas, &joins, &pieces};
-  return paged_launch(f16 ? finish_of<F16>(d) : finish_of<Bf16>(d), dim3(joins + weighs), dim3(kThreads), 0, 1, left, stream);
+  return paged_launch(f16 ? finish_of<F16>(d) : finish_of<Bf16>(d), dim3(joins + weighs), dim3(kThreads), 0, 0, 1, left, stream);
 }

@@ -990,7 +990,8 @@ uint32_t cluster_for(uint64_t items, uint64_t longest, uint32_t worth, size_t ke
 }
 
 constexpr size_t kRoom = 196 * 1024;
-constexpr size_t kPagesRoom = 58 * 1024;   // beside the ring and q's operands (24 KiB at most)
+constexpr size_t kOperands = 24 * 1024;    // q's, at most
+constexpr size_t kPagesRoom = 58 * 1024;   // beside the ring and those
 template <class T, int D>
 const void* select_of(bool many) {
   return many ? (const void*)select_kernel<T, D, 8> : (const void*)select_kernel<T, D, 4>;
@@ -1040,7 +1041,8 @@ extern "C" fz_status fz_paged_select(const fz_paged_kv* kv, const float* q, uint
                           : d == 128 ? select_of<Bf16, 128>(many)
                                      : select_of<Bf16, 256>(many));
   return paged_launch(fn, dim3((uint32_t)(items * c)), dim3(kThreads),
-                      kRing + d / 8 * tiles * 256 + slice * 8 + all * 4 + (all + 31) / 32 * 4, c, args, stream);
+                      kRing + d / 8 * tiles * 256 + slice * 8 + all * 4 + (all + 31) / 32 * 4, kRing + kOperands + kPagesRoom, c, args,
+                      stream);
 }
 
 extern "C" fz_status fz_paged_evict(const fz_paged_kv* from, const fz_paged_kv* to, uint32_t budget, uint32_t sink,
@@ -1070,13 +1072,13 @@ extern "C" fz_status fz_paged_evict(const fz_paged_kv* from, const fz_paged_kv* 
   a.budget = budget, a.sink = sink, a.recent = recent, a.kept = kept;
   uint32_t slice = (uint32_t)((longest + c - 1) / c);
   void* args[] = {&a, &slice};
-  if ((st = paged_launch((const void*)keep_kernel, dim3((uint32_t)(items * c)), dim3(kThreads), slice * 4, c, args, stream)))
+  if ((st = paged_launch((const void*)keep_kernel, dim3((uint32_t)(items * c)), dim3(kThreads), slice * 4, kRoom, c, args, stream)))
     return st;
   void* move[] = {&a};
   const uint32_t rows = 8 * 4 * (256 / from->head_dim);    // a CTA's entries
   const void* fn = from->head_dim == 64    ? (const void*)move_kernel<64>
                    : from->head_dim == 128 ? (const void*)move_kernel<128>
                                            : (const void*)move_kernel<256>;
-  return paged_launch(fn, dim3((uint32_t)((std::min<uint64_t>(budget, longest) + rows - 1) / rows), (uint32_t)items), dim3(256), 0, 1,
+  return paged_launch(fn, dim3((uint32_t)((std::min<uint64_t>(budget, longest) + rows - 1) / rows), (uint32_t)items), dim3(256), 0, 0, 1,
                       move, stream);
 }

@@ -221,3 +221,41 @@ def test_evict_leaves_out_entries_of_bad_pages(kv, lengths, bad, budget, sink, r
     got = attend(b, q, 0.125)
     want, _, bound = attend_exact(b, q, 0.125)
     assert ((got.double() - want).abs() <= bound).all()
+
+
+# ------------------------------------------------------------------ host threads
+
+@pytest.mark.parametrize("op", ["select", "evict"])
+def test_two_host_threads_with_tables_of_unlike_widths(op):
+    """Calls of caches with long and short tables from two threads at once: each call's need of shared memory is its own."""
+    torch = torch_cuda()
+    lib = _native.load()
+    jobs = []
+    for i, capacity in enumerate([20000, 4500] if op == "select" else [400000, 40000]):
+        cache = Cache([4], page=1 if op == "select" else 4, d=64, weights=True, bounds=True, seed=i, capacity=capacity)
+        to = Cache([4], page=4, d=64, weights=True, seed=9)
+        q = randn(1, 1, 64)
+        blocks, kept = (torch.zeros(1, 1, 4, dtype=torch.int32, device="cuda") for _ in range(2))
+        jobs.append((cache, to, q, blocks, kept, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    failed = [[], []]
+    start = threading.Barrier(2)
+
+    def calls(i):
+        cache, to, q, blocks, kept, st = jobs[i]
+        start.wait()
+        for _ in range(3000):
+            if op == "select":
+                status = lib.fz_paged_select(cache.desc, q.data_ptr(), 64, 1, 4, 0, 0, blocks.data_ptr(), None, st.cuda_stream)
+            else:
+                status = lib.fz_paged_evict(cache.desc, to.desc, 4, 0, 0, kept.data_ptr(), st.cuda_stream)
+            if status:
+                failed[i].append((status, lib.fz_last_error()))
+
+    threads = [threading.Thread(target=calls, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed[0] and not failed[1], (len(failed[0]), len(failed[1]), (failed[0] + failed[1])[0])
