@@ -952,12 +952,19 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   const uint32_t tile = 4096 / kv->head_dim;
   const uint64_t tiles = (most + tile - 1) / tile;
   // Items stay whole, by their number alone (no CTA needs every length, and
-  // nothing is left to add up), where they have at most a tile a warp, or where
-  // even items of the longest list take no longer than cut ones (64 sequences of
-  // 2 KV heads and a window of 512: 14.4 us cut or left whole by their lengths,
-  // 11.0 so).
-  const double cost = (double)tiles + kWarps, rounds = (double)((items + kCtas - 1) / kCtas);
-  a.whole = tiles <= kWarps || rounds * cost <= (double)items / kCtas * cost + 2 * kJoin;
+  // nothing is left to add up), where they have at most a tile a warp, or where a
+  // CTA's whole items are at most eight tiles a warp and an even share would save
+  // less than the joining costs.  The longest list there may be decides that, not
+  // the lengths there are, so it holds only as far as whole items are no slower for
+  // one list that long beside short ones either: 148 sequences of d = 256 over tables
+  // of 512 entries, all full 13.2 us whole, 16.3 cut by their lengths, one full
+  // beside others of 20 entries 12.3 and 19.9; 296 of them 30.3 and 34.2, 16.2 and
+  // 20.3; 148 of 1,024 entries 28.7 and 32.3, 19.1 and 19.8; of 2,048 52 and 55, but
+  // 32.5 and 19.9 (of 32,768 more than twenty times as long); 64 sequences of 2 KV
+  // heads and a window of 512 9.5 and 12.4, one of them full 9.0 and 12.0.
+  const uint64_t rounds = (items + kCtas - 1) / kCtas;
+  a.whole = tiles <= kWarps || (rounds * tiles <= 8 * kWarps &&
+                                (rounds * kCtas - items) * (tiles + kWarps) <= 2ull * kJoin * kCtas);
   const uint32_t grid =
       (uint32_t)std::min<uint64_t>(kCtas, a.whole ? items : (items * tiles + kWarps - 1) / kWarps);
   a.recip = grid > 1 ? ~0ull / grid + 1 : 0;

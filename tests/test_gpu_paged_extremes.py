@@ -259,3 +259,43 @@ def test_two_host_threads_with_tables_of_unlike_widths(op):
         t.join()
     torch.cuda.synchronize()
     assert not failed[0] and not failed[1], (len(failed[0]), len(failed[1]), (failed[0] + failed[1])[0])
+
+
+def test_one_long_list_among_many_short_ones():
+    """The long sequence's list is cut over the GPU whatever else the batch holds: 147 short ones beside it cost less than
+    four times its own time (on one SM it takes more than twenty times that)."""
+    torch = torch_cuda()
+
+    def run(lengths):
+        cache = long_cache(lengths)
+        q = randn(len(lengths), 4, 256, seed=1)
+        space = torch.empty(_native.load().fz_paged_attention_workspace(cache.desc, 4), dtype=torch.uint8, device="cuda")
+        out = torch.empty_like(q)
+        best = float("inf")
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(5):
+                attend(cache, q, 0.0625, workspace=space, out=out)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        want, _, bound = attend_exact(cache, q, 0.0625)
+        assert ((out.double() - want).abs() <= bound).all()
+        return best
+
+    def long_cache(lengths):
+        """Tables of 32,768 entries over a pool that holds only what the sequences do."""
+        cache = Cache([max(lengths)] + [200], page=16, d=256, seed=4)
+        table = np.full((len(lengths), 32768 // 16), 0xFFFFFFFF, dtype=np.uint32)
+        for s, n in enumerate(lengths):
+            table[s, :(n + 15) // 16] = cache.table_np[0 if n == max(lengths) else 1, :(n + 15) // 16]
+        cache.lengths, cache.table_np = lengths, table
+        cache.table, cache.len = Cache.u32(table), Cache.u32(np.array(lengths, dtype=np.uint32))
+        cache.desc.page_table, cache.desc.lengths = cache.table.data_ptr(), cache.len.data_ptr()
+        cache.desc.sequences, cache.desc.table_stride = len(lengths), table.shape[1]
+        return cache
+
+    alone = run([32768])
+    among = run([200] * 70 + [32768] + [200] * 77)
+    assert among < 4 * alone, (among, alone)
