@@ -878,9 +878,13 @@ const void* finish_of(uint32_t d) {
                     : (const void*)finish_kernel<T, 256>;
 }
 
-// Where each part of the workspace begins; returns its whole size.
+// Where each part of the workspace begins; returns its whole size, kTooLarge
+// from 2^62 bytes on.
+constexpr size_t kTooLarge = ~(size_t)0;
 size_t layout(const fz_paged_kv* kv, uint32_t heads, size_t (&at)[6]) {
   const uint64_t group = heads / std::max(1u, kv->kv_heads), items = (uint64_t)kv->sequences * kv->kv_heads;
+  const double scores = (double)items * ((double)kv->table_stride * kv->page_slots + kWeighed) * group * 4;
+  if ((kv->weights && scores >= 0x1p62) || (double)group * kv->head_dim >= 0x1p40) return kTooLarge;
   const uint64_t entries = ((uint64_t)kv->table_stride * kv->page_slots + kWeighed - 1) / kWeighed * kWeighed;
   const uint64_t bytes[6] = {kCtas * 2ull * group * kv->head_dim * 4, kCtas * 2ull * 8 * 8, kCtas * 16ull,
                              kv->weights ? items * 16 : 0, kv->weights ? items * 64 : 0,
@@ -923,7 +927,7 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   if (query->blocks && query->top == 0) return paged_refuse(FZ_ERR_ARGUMENT, "selected pages need top nonzero");
   if (reinterpret_cast<uintptr_t>(query->blocks) & 3u) return paged_refuse(FZ_ERR_ARGUMENT, "blocks not 4-byte aligned");
   const size_t need = fz_paged_attention_workspace(kv, heads);
-  if (!query->workspace || (reinterpret_cast<uintptr_t>(query->workspace) & 255u) || query->workspace_bytes < need)
+  if (need == kTooLarge || !query->workspace || (reinterpret_cast<uintptr_t>(query->workspace) & 255u) || query->workspace_bytes < need)
     return paged_refuse(FZ_ERR_ARGUMENT, "workspace null, not 256-byte aligned, or shorter than fz_paged_attention_workspace");
   const uint64_t items = (uint64_t)kv->sequences * kv->kv_heads;
   if (items > 0x7FFFFFFFull) return paged_refuse(FZ_ERR_ARGUMENT, "too many sequences");

@@ -578,7 +578,7 @@ typedef struct fz_paged_query {
 } fz_paged_query;
 fz_status fz_paged_attention(const fz_paged_kv *kv, const fz_paged_query *query, void *stream);
 /* Bytes of workspace for the cache as described and `heads` query heads: a few MiB, with kv->weights 4 more a query
- * head and table entry. */
+ * head and table entry; SIZE_MAX, which no call takes, from 2^62 bytes on. */
 size_t fz_paged_attention_workspace(const fz_paged_kv *kv, uint32_t heads);
 
 /* Keeps at most `budget` entries of each sequence and KV head and writes them,
