@@ -44,6 +44,9 @@ fz_status paged_view(const fz_paged_kv* kv, uint32_t need, PagedView* out) {
   if (!kv->kv_heads || !kv->page_slots || !kv->pages || !kv->table_stride)
     return paged_refuse(FZ_ERR_ARGUMENT, "kv_heads, page_slots, pages and table_stride must be nonzero");
   if (kv->kv_heads > 65535) return paged_refuse(FZ_ERR_ARGUMENT, "more than 65,535 KV heads");
+  // (Counters of 32 bits run over them in steps.)
+  if ((uint64_t)kv->sequences * kv->kv_heads > 0x7FFFFFFFull)
+    return paged_refuse(FZ_ERR_ARGUMENT, "more than 2^31 - 1 sequences times KV heads");
   if ((uint64_t)kv->table_stride * kv->page_slots > (1u << 30))
     return paged_refuse(FZ_ERR_ARGUMENT, "a table of more than 2^30 entries a sequence");
   if (!kv->page_table || !kv->lengths) return paged_refuse(FZ_ERR_ARGUMENT, "null page table or lengths");

@@ -930,7 +930,6 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   if (need == kTooLarge || !query->workspace || (reinterpret_cast<uintptr_t>(query->workspace) & 255u) || query->workspace_bytes < need)
     return paged_refuse(FZ_ERR_ARGUMENT, "workspace null, not 256-byte aligned, or shorter than fz_paged_attention_workspace");
   const uint64_t items = (uint64_t)kv->sequences * kv->kv_heads;
-  if (items > 0x7FFFFFFFull) return paged_refuse(FZ_ERR_ARGUMENT, "too many sequences");
   if (items == 0) return FZ_OK;
   const void* p[] = {kv->keys, kv->values, kv->page_table, kv->lengths, kv->weights, kv->error,
                      query->q, query->out, query->blocks,  query->workspace};

@@ -990,6 +990,7 @@ uint32_t cluster_for(uint64_t items, uint64_t longest, uint32_t worth, size_t ke
 }
 
 constexpr size_t kRoom = 196 * 1024;
+constexpr uint32_t kMostListed = 1u << 30; // as many as a table may have (counters of 32 bits run over lists in steps)
 constexpr size_t kOperands = 24 * 1024;    // q's, at most
 constexpr size_t kPagesRoom = 58 * 1024;   // beside the ring and those
 template <class T, int D>
@@ -1015,6 +1016,7 @@ extern "C" fz_status fz_paged_select(const fz_paged_kv* kv, const float* q, uint
     return paged_refuse(FZ_ERR_ARGUMENT, "heads must be 1 to 8 times kv_heads");
   if (kv->sequences > 1 && q_stride < (uint64_t)heads * kv->head_dim)
     return paged_refuse(FZ_ERR_ARGUMENT, "a q stride shorter than its heads");
+  if (top > kMostListed) return paged_refuse(FZ_ERR_ARGUMENT, "top of more than 2^30");
   if (top == 0 || (uint64_t)sink + recent > top) return paged_refuse(FZ_ERR_ARGUMENT, "top must be nonzero and at least sink + recent");
   const uint64_t items = (uint64_t)kv->sequences * kv->kv_heads;
   const uint32_t c = cluster_for(items, kv->table_stride, 32, 13, kPagesRoom);
@@ -1058,6 +1060,7 @@ extern "C" fz_status fz_paged_evict(const fz_paged_kv* from, const fz_paged_kv* 
     return paged_refuse(FZ_ERR_ARGUMENT, "from and to differ in type, sequences, KV heads or head dimension");
   if (budget == 0 || (uint64_t)sink + recent > budget)
     return paged_refuse(FZ_ERR_ARGUMENT, "budget must be nonzero and at least sink + recent");
+  if (budget > kMostListed) return paged_refuse(FZ_ERR_ARGUMENT, "budget of more than 2^30");
   const uint64_t longest = (uint64_t)from->table_stride * from->page_slots, room = (uint64_t)to->table_stride * to->page_slots;
   if (std::min<uint64_t>(budget, longest) > room) return paged_refuse(FZ_ERR_ARGUMENT, "budget past the destination's table");
   const uint64_t items = (uint64_t)from->sequences * from->kv_heads;

@@ -468,7 +468,9 @@ fz_status fz_attention_static(const float *q, const void *key_cache, const void 
  * of an entry that takes part gives infinities or NaN.  Pages that several
  * sequences share may be read by all of them (fz_paged_bounds too, where each
  * holds them whole); fz_paged_append, weight accumulation and fz_paged_evict's
- * `to` want pages of one sequence only.
+ * `to` want pages of one sequence only.  At most 2^30 entries a sequence by its
+ * table, 2^31 - 1 sequences times KV heads, and 2^30 words a list (`top`,
+ * `budget`).
  *
  * Lengths, tables and rows are device memory, so the host cannot check them:
  * the kernels do.  What they find out of range is skipped, never followed,
