@@ -531,10 +531,12 @@ FZ_DEV uint32_t greater_size<Bf16>(uint32_t m, uint32_t x) {
 // of q, bf16 24).  The order of the 2 D products is free, so a lane takes 16
 // bytes of a row as they lie for two steps' A operands; it copies them itself,
 // by cp.async three stages ahead, and no barrier or ldmatrix comes between.  Two
-// MMAs run into one f32 sum (32 additions to at least single precision, 2^-23 of
-// the products' sizes each), those are added in f32 (2 D / 32 of them, and at
-// most four of parts): 64 + 20 times 2^-24; what q's parts leave out is 2^-23 of a
-// value, or 2^-25 of the head's largest where a remainder is subnormal.
+// MMAs run into one f32 sum: 32 additions, each taken to be within 2^-23 of the
+// products' sizes, which is an assumption (the instruction's rounding is not
+// documented; over products of all sizes that cancel, all 32 together were off by
+// 0.3 x 2^-23 of the sizes at most).  Those sums are added in f32 (2 D / 32 of them,
+// and at most four of parts): 64 + 20 times 2^-24; what q's parts leave out is 2^-23
+// of a value, or 2^-25 of the head's largest where a remainder is subnormal.
 //
 // A product may be lost below the least normal f32: the 3 D that are not zero are
 // less than 2^-24 of a head's size with bounds of 10^-26, so E takes no smaller

@@ -465,12 +465,12 @@ fz_status fz_attention_static(const float *q, const void *key_cache, const void 
  * i slot_stride + h head_stride, in elements, head_dim elements in a row.  So
  * slot-major and head-major pages are both only strides.  Slots past a
  * sequence's length are never read, whatever they hold.  An infinite key or value
- * of an entry that takes part gives infinities or NaN.  Pages that several
- * sequences share may be read by all of them (fz_paged_bounds too, where each
- * holds them whole); fz_paged_append, weight accumulation and fz_paged_evict's
- * `to` want pages of one sequence only.  At most 2^30 entries a sequence by its
- * table, 2^31 - 1 sequences times KV heads, and 2^30 words a list (`top`,
- * `budget`).
+ * of an entry that takes part, or a score past the largest f32, gives infinities
+ * or NaN.  Pages that several sequences share may be read by all of them
+ * (fz_paged_bounds too, where each holds them whole); fz_paged_append, weight
+ * accumulation and fz_paged_evict's `to` want pages of one sequence only.  At
+ * most 2^30 entries a sequence by its table, 2^31 - 1 sequences times KV heads,
+ * and 2^30 words a list (`top`, `budget`).
  *
  * Lengths, tables and rows are device memory, so the host cannot check them:
  * the kernels do.  What they find out of range is skipped, never followed,
@@ -513,10 +513,11 @@ typedef struct fz_paged_kv {
  * (NULL: not rotated; a pair with turns 0 stays).  The rotation is taken from
  * the 64-bit product's fraction, so positions of any size keep f32 angles
  * (rope.wgsl:120-138 reduces the f32 product).  Queries go to q_out as f32,
- * which may be q itself; keys and values into the pages, rounded to nearest
- * even, f16 saturating at +-65,504 (f16_pack.wgsl:16-19).  An appended entry's
- * accumulated weight becomes 0, and lengths[s] grows to index + 1 where that
- * is more.  Two rows of one call must not name the same entry. */
+ * which may be q itself with q's stride; keys and values into the pages,
+ * rounded to nearest even, f16 saturating at +-65,504 (f16_pack.wgsl:16-19).
+ * An appended entry's accumulated weight becomes 0, and lengths[s] grows to
+ * index + 1 where that is more.  Two rows of one call must not name the same
+ * entry. */
 typedef struct fz_paged_rows {
   const float *q, *k, *v;       /* [rows][heads or kv_heads][head_dim], 16-byte aligned */
   float *q_out;                 /* [rows][heads][head_dim] */
@@ -547,9 +548,9 @@ fz_status fz_paged_bounds(const fz_paged_kv *kv, const uint32_t *first, void *st
  * last `recent` pages are taken first (sink + recent <= top), then the best
  * scores, equal ones by the lower page, NaN before all numbers.  q as in
  * fz_paged_attention.  scores: NULL or [sequences][kv_heads][top], each
- * listed page's score rounded to f32 (0 past them; pages that are none come
- * last, and where one is listed all the same its score is -infinity).  Keys and
- * values are not read. */
+ * listed page's score rounded to f32 (0 past them).  Pages that are none come
+ * after all others, unless taken first, and where one is listed its score is
+ * -infinity.  Keys and values are not read. */
 fz_status fz_paged_select(const fz_paged_kv *kv, const float *q, uint64_t q_stride, uint32_t heads, uint32_t top,
                           uint32_t sink, uint32_t recent, uint32_t *blocks, float *scores, void *stream);
 

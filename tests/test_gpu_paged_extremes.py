@@ -91,6 +91,37 @@ def test_attention_query_with_one_large_dimension(type, heads, d, outlier):
     assert ((got.double() - want).abs() <= bound).all(), float(((got.double() - want).abs() / bound).max())
 
 
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_sums_of_products_within_the_units_assumed(type):
+    """The tensor cores' f32 sums, which the margin of fz_paged_select and the bounds of attend_exact rest on: each of the
+    32 additions of two steps of 16 products within 2^-23 of the products' sizes.  Products of every size that cancel to
+    nothing, in the dimensions that one of the attention's sums takes, read from the weight of a key against one of
+    zero: out[1] / out[0] = e^(scale q k)."""
+    torch = torch_cuda()
+    S, d, G = 400, 256, 4
+    rng = np.random.default_rng(7)
+    steps = np.r_[0:16, 64:80]                                       # step 0 and step 4, of one sum
+    k = np.zeros((S, d))
+    for s in range(S):
+        spread = rng.choice([2, 8, 14, 20])                          # (f16 holds them all as normal numbers)
+        half = (1.0 + rng.integers(0, 128, 16) / 128.0) * 2.0 ** (14 - rng.integers(0, spread + 1, 16)) * rng.choice([-1, 1], 16)
+        k[s, steps] = rng.permutation(np.concatenate([half, -half]))
+    cache = Cache([2] * S, page=2, d=d, type=type)
+    cache.keys.zero_()
+    cache.values.zero_()
+    rows = torch.from_numpy(cache.table_np[:, 0].astype(np.int64)).cuda()
+    cache.keys[rows, 1, 0] = torch.from_numpy(k).cuda().to(cache.dtype)
+    cache.values[rows, 0, 0, 0] = 1.0
+    cache.values[rows, 1, 0, 1] = 1.0
+    assert (cache.keys[rows, 1, 0].double().cpu().numpy() == k).all()
+    size = float(np.abs(k).sum(1).max())
+    scale = 2.0 ** 18 / size                                         # a unit of 32 x 2^-23 of the largest size: 1
+    out = attend(cache, torch.ones(S, G, d, device="cuda"), scale).double()
+    score = torch.log(out[..., 1] / out[..., 0]).abs().amax(1).cpu().numpy()
+    # (the weights are within 2^-20, and the factor of the scores within 2^-23 of their size)
+    assert (score <= 32 * 2.0 ** -23 * np.abs(k).sum(1) * scale + 2.0 ** -19).all(), score.max()
+
+
 # ------------------------------------------------------------------ selection
 
 def check_scores(cache, q, blocks, scores, size=None):
