@@ -122,9 +122,10 @@ FZ_DEV Parts<T> parts(float x, float y, float lift = 1.f) {
   return p;
 }
 // A query is divided by 2^(e - 127), of its largest value `top`: to [1, 2) for
-// f16 keys, to 2^-10 of that for bf16 ones, which may be as large as an f32, so
-// that no sum of up to 256 products overflows by the way (2^8 x 2^-9 x the
-// largest key).  2^(e - 127) and its reciprocal are normal.
+// f16 keys (2^14 times that in attend_kernel), to 2^-10 of that for bf16 ones,
+// which may be as large as an f32, so that no sum of up to 256 products overflows
+// by the way (2^8 x 2^-9 x the largest key).  2^(e - 127) and its reciprocal are
+// normal.
 template <class T>
 FZ_DEV uint32_t query_exponent(float top) {
   return min(max(__float_as_uint(top) >> 23, 1u) + (T::kType == FZ_KV_F16 ? 0u : 10u), 253u);

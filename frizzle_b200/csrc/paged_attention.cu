@@ -273,12 +273,11 @@ FZ_DEV float unit_of(uint32_t count) {
 // that its largest is about 2^14, and the remainders of f16 parts, q's and the
 // weights', are times 2^11 more: q keeps 22 bits down to 2^-28 of a head's largest
 // (one far larger dimension costs the others nothing) and 2^-50 of that below; the
-// weights, at unit_of, 22 bits and 2^-51 of the largest.  (f32's own 24
-// bits would take one MMA more a step; 2^-22 of a score's products' sizes is less
-// than its f32 sum may be off by.)  A
-// tile's product starts from zero and is added to the running output in f32 (the
-// fold's multiply-add), so the tensor cores' own accumulation never runs along
-// the sequence.
+// weights, at unit_of, 22 bits and 2^-51 of the largest.  (f32's own 24 bits would
+// take one MMA more a step; 2^-22 of a score's products' sizes is less than its f32
+// sum may be off by.)  A tile's product starts from zero and is added to the running
+// output in f32 (the fold's multiply-add), so the tensor cores' own accumulation
+// never runs along the sequence.
 //
 // Bound by HBM: 2 x d x 2 bytes an entry, G x 4 flops a byte.  So each warp is a
 // stream of its own: it copies its tiles (8 KiB of keys, 8 of values: 4096 / d
@@ -293,7 +292,7 @@ FZ_DEV float unit_of(uint32_t count) {
 // Measured with it, d = 256, 4 heads, f16 (one CTA a sequence and KV head with
 // f32 products: 13.3 ms for the first): 8 sequences of up to 32,768 entries, 193
 // MB, 38 us (5.1 TB/s), 44 with their weights; up to 131,072 entries 125 us (6.2
-// TB/s); 2,048 selected entries of each 10.8 us; one of 36 entries 6.0 us, of
+// TB/s); 2,048 selected entries of each 10.9 us; one of 36 entries 5.7 us, of
 // 4,096 9.4 us, some ten dependent reads, barriers and launches.
 template <class T, int D, int GP>
 __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a) {
@@ -329,8 +328,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
   pdl_wait();
   pdl_launch_dependents();
 
-  // This CTA's items: a share of all units, or where no item has more than one
-  // tile a warp, whole items by their number alone.
+  // This CTA's items: a share of all units, or where lists are short (as the host
+  // decides) whole items by their number alone.
   Walk seg{};
   uint32_t units = 0x7FFFFFFFu, items = 0xFFFFFFFFu, last_item = 0xFFFFFFFFu, extra = 0;
   uint64_t first = 0, per = 1;
@@ -704,11 +703,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a)
 // in a fixed order, so the sum never depends on who came first.
 //
 // The others make the entries' weights from the scores and the items' maxima
-// and sums, exp2(score - maximum) / sum (the maximum as it is: one
-// lifted with the weights' unit would be rounded from 2^24 on), 128 entries a warp at a time, four a lane, each entry written by the
-// one lane it falls to.  (Without the bound on the CTAs an SM some forms were
-// compiled to 80 registers and spilled: 10.8 -> 11.2 us for 2,048 selected entries
-// of 8 sequences.)
+// and sums, exp2(score - maximum) / sum (the maximum as it is: one lifted with the
+// weights' unit would be rounded from 2^24 on), 128 entries a warp at a time, four
+// a lane, each entry written by the one lane it falls to.  (Without the bound on
+// the CTAs an SM some forms were compiled to 80 registers and spilled: 10.8 -> 11.2
+// us for 2,048 selected entries of 8 sequences.)
 constexpr int kWeighed = 128;
 template <class T, int D>
 __global__ void __launch_bounds__(kThreads, 2) finish_kernel(const AttendArgs a, uint32_t ctas, uint32_t joins, uint32_t pieces) {
@@ -964,7 +963,10 @@ extern "C" fz_status fz_paged_attention(const fz_paged_kv* kv, const fz_paged_qu
   // beside others of 20 entries 12.3 and 19.9; 296 of them 30.3 and 34.2, 16.2 and
   // 20.3; 148 of 1,024 entries 28.7 and 32.3, 19.1 and 19.8; of 2,048 52 and 55, but
   // 32.5 and 19.9 (of 32,768 more than twenty times as long); 64 sequences of 2 KV
-  // heads and a window of 512 9.5 and 12.4, one of them full 9.0 and 12.0.
+  // heads and a window of 512 9.5 and 12.4, one of them full 9.0 and 12.0.  At most a
+  // tile a warp: 1,184 sequences over tables of 128 entries, all full 45 and 49, an
+  // eighth full beside others of 2 entries 41 and 65; beside empty ones 58 and 28,
+  // which is the one kind of batch that loses.
   const uint64_t rounds = (items + kCtas - 1) / kCtas;
   a.whole = tiles <= kWarps || (rounds * tiles <= 8 * kWarps &&
                                 (rounds * kCtas - items) * (tiles + kWarps) <= 2ull * kJoin * kCtas);
