@@ -194,6 +194,34 @@ def test_select_scores_with_bounds_infinite_on_the_side_not_picked(heads, length
     assert torch.isfinite(scores[0, 0, [2, 4]]).all() and scores[0, 0, 3] == float("inf")
 
 
+@pytest.mark.parametrize("type,q_scale,bound", [
+    ("bf16", 1e-5, 3e38), ("bf16", 1e37, 1e-38), ("bf16", 1e-41, 1.0), ("bf16", 1e-41, 1e38), ("bf16", 1e38, 3e38), ("bf16", 1.0, 1e-39),
+    ("f16", 1e-41, 1.0), ("f16", 1e34, 6e4), ("f16", 1e-36, 1e-6), ("f16", 1e-43, 1e-7)])
+def test_select_scores_at_the_ends_of_f32(type, q_scale, bound):
+    """Queries and bounds below the least normal f32, scores past the largest and below the least."""
+    torch = torch_cuda()
+    cache = Cache([600 * 16, 40], page=16, d=128, kv=2, type=type, bounds=True)
+    b = torch.rand(cache.bounds.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) * 2 - 1
+    cache.bounds.copy_(torch.sort(b, dim=2).values * bound)
+    q = torch.clamp(randn(2, 6, 128, seed=6), -3, 3) * q_scale
+    check_scores(cache, q, *select(cache, q, 60))
+
+
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("heads", [1, 3, 8])
+def test_select_scores_of_queries_without_a_number(heads, value):
+    """Beside pages whose bounds are infinite, NaN or zero."""
+    cache = Cache([100 * 16], page=16, d=256, bounds=True)
+    bounds(cache)
+    q = randn(1, heads, 256)
+    q[0, heads // 2, 3] = value
+    cache.bounds[int(cache.table_np[0, 2]), 0, 1, 3] = float("inf")
+    cache.bounds[int(cache.table_np[0, 4]), 0, :, 4] = float("nan")
+    cache.bounds[int(cache.table_np[0, 6]), 0, :, 3] = 0.0
+    check_scores(cache, q, *select(cache, q, 100))
+    check_scores(cache, q, *select(cache, q, 9, 7, 1))
+
+
 @pytest.mark.parametrize("pages,take", [(11, 11), (11, 6), (3000, 40)])
 def test_select_score_of_a_page_that_is_none(pages, take):
     """-infinity, below every other page's."""
